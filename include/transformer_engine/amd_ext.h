@@ -87,6 +87,60 @@ void nvte_amd_multi_gemm(const NVTETensor *A, const NVTETensor *B, NVTETensor *D
                          const int *transb, int num_gemms, int grad, NVTETensor workspace, const int *accumulate,
                          hipStream_t stream);
 
+/* ---- Global gradient norm and clipping over a list of tensors (Python: weight_update.grad_norm, clip_grad_norm).
+ * norm = sqrt(sum of squares of every element of every tensor), squares summed in 64 bits in a fixed order.
+ * grads[i] is a device array of numels[i] elements of NVTEDType dtypes[i] (fp32 / fp16 / bf16, mixed at will); empty
+ * tensors count nothing.  The lists themselves are host arrays.  Inf and NaN run through: the norm is then Inf or NaN. */
+size_t nvte_amd_grad_norm_workspace_size(const size_t *numels, size_t num_tensors);
+/* *sum_of_squares (fp64) and *norm (fp32), device pointers; either may be NULL */
+void nvte_amd_grad_norm(const void *const *grads, const size_t *numels, const int *dtypes, size_t num_tensors,
+                        double *sum_of_squares, float *norm, void *workspace, size_t workspace_bytes, hipStream_t stream);
+/* outs[i] = grads[i] * min(1, max_norm / (norm + eps)), rounded once to out_dtypes[i]; *norm as above.  outs[i] may be
+ * grads[i] itself (in place, one dtype); any other overlap of an output with a tensor of the call is an error. */
+void nvte_amd_clip_grad_norm(const void *const *grads, void *const *outs, const size_t *numels, const int *dtypes,
+                             const int *out_dtypes, size_t num_tensors, float max_norm, float eps, float *norm,
+                             void *workspace, size_t workspace_bytes, hipStream_t stream);
+/* The second half alone, for a sum of squares that was added up over ranks first. */
+void nvte_amd_clip_by_sum_of_squares(const void *const *grads, void *const *outs, const size_t *numels, const int *dtypes,
+                                     const int *out_dtypes, size_t num_tensors, const double *sum_of_squares,
+                                     float max_norm, float eps, float *norm, hipStream_t stream);
+
+/* ---- Low-rank adapters of many requests beside a shared projection (Python: lora.py).
+ * x [tokens, in], a [num_adapters, rank, in], b [num_adapters, out, rank], base / out [tokens, out], all of one dtype (bf16 or
+ * fp16), contiguous; adapter_ids [tokens] int32, any order, a value outside [0, num_adapters) = no adapter; scaling
+ * [num_adapters] fp32 or NULL (1); base NULL = zero, or out itself.  rank 1 to 128, any feature sizes.
+ *   low[t] = a[id] x[t]        out[t] = base[t] + scaling[id] b[id] low[t]
+ * low [nvte_amd_lora_num_slices(tokens, in), tokens, rank] fp32: partial sums of the rank vectors, which the backward pass reads
+ * (rows without an adapter are not written).  A non-finite weight or activation makes its own rows non-finite and no other. */
+size_t nvte_amd_lora_num_slices(size_t tokens, size_t features);
+void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const int *adapter_ids, const float *scaling,
+                           const void *base, void *out, float *low, size_t tokens, size_t in_features, size_t out_features,
+                           size_t rank, size_t num_adapters, int dtype, hipStream_t stream);
+/* dx[t] = base_grad[t] + scaling[id] a[id]^T (b[id]^T dy[t]); da [num_adapters, rank, in] and db [num_adapters, out, rank], in
+ * dtype or fp32 (grad_dtype), are sums over each adapter's tokens in a fixed order, zero for an adapter without tokens.  dx may
+ * be NULL, da and db may be NULL together; base_grad NULL = zero, or dx itself.  Up to 4096 adapters when da / db are wanted. */
+size_t nvte_amd_lora_backward_workspace_size(size_t tokens, size_t in_features, size_t out_features, size_t rank,
+                                             size_t num_adapters);
+void nvte_amd_lora_backward(const void *x, const void *dy, const void *a, const void *b, const int *adapter_ids,
+                            const float *scaling, const float *low, const void *base_grad, void *dx, void *da, void *db,
+                            size_t tokens, size_t in_features, size_t out_features, size_t rank, size_t num_adapters,
+                            int dtype, int grad_dtype, void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- A mixture-of-experts layer for a few tokens (Python: moe.py); larger batches: the grouped GEMM.
+ * Router: p = softmax(logits[t]) over num_experts (<= 1024) fp32 / fp16 / bf16 logits; topk_ids [tokens, top_k] int32 = the largest,
+ * in falling order, ties to the lowest index, NaN last; topk_weights fp32 = p of them, divided by their sum if renormalize. */
+void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, size_t tokens, size_t num_experts, size_t top_k,
+                       int renormalize, int dtype, hipStream_t stream);
+/* out[t] = sum_j topk_weights[t, j] w_fc2[e] (silu(w_fc1[e][:ffn] x[t]) * (w_fc1[e][ffn:] x[t])), e = topk_ids[t, j]; an id
+ * outside [0, num_experts) adds nothing.  x, out [tokens, hidden] bf16 or fp16; w_fc1 [num_experts, 2 ffn, hidden] and w_fc2
+ * [num_experts, hidden, ffn] of the same dtype, or FP8 E4M3 with one fp32 scale_inv per expert.  Up to 256 tokens, top_k up to
+ * 64, tokens * top_k up to 4096.  out must not overlap an input. */
+size_t nvte_amd_moe_forward_workspace_size(size_t tokens, size_t top_k, size_t num_experts, size_t hidden, size_t ffn);
+void nvte_amd_moe_forward(const void *x, const void *w_fc1, const void *w_fc2, const float *fc1_scale_inv,
+                          const float *fc2_scale_inv, const int *topk_ids, const float *topk_weights, void *out,
+                          size_t tokens, size_t top_k, size_t num_experts, size_t hidden, size_t ffn, int dtype,
+                          int weight_dtype, void *workspace, size_t workspace_size, hipStream_t stream);
+
 /* Library identification: "transformerengine_amd <version> gfx950". */
 const char *nvte_amd_version(void);
 

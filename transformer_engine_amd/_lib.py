@@ -116,6 +116,17 @@ _SIGS = {
     "nvte_amd_get_columnwise_transposed": (_I, [_P]),
     "nvte_amd_delayed_scaling_after_reduction": (_V, [_P, C.POINTER(_P), C.POINTER(_P), _SZ, C.c_char_p, _I, _F, _P]),
     "nvte_amd_delayed_scaling_after_reduction_multi": (_V, [_P, C.POINTER(_P), C.POINTER(_P), C.POINTER(_I), _SZ, C.c_char_p, _F, _P]),
+    "nvte_amd_grad_norm_workspace_size": (_SZ, [_P, _SZ]),
+    "nvte_amd_grad_norm": (_V, [_P, _P, _P, _SZ, _P, _P, _P, _SZ, _P]),
+    "nvte_amd_clip_grad_norm": (_V, [_P, _P, _P, _P, _P, _SZ, _F, _F, _P, _P, _SZ, _P]),
+    "nvte_amd_clip_by_sum_of_squares": (_V, [_P, _P, _P, _P, _P, _SZ, _P, _F, _F, _P, _P]),
+    "nvte_amd_lora_num_slices": (_SZ, [_SZ, _SZ]),
+    "nvte_amd_lora_forward": (_V, [_P] * 8 + [_SZ] * 5 + [_I, _P]),
+    "nvte_amd_lora_backward_workspace_size": (_SZ, [_SZ] * 5),
+    "nvte_amd_lora_backward": (_V, [_P] * 11 + [_SZ] * 5 + [_I, _I, _P, _SZ, _P]),
+    "nvte_amd_moe_topk": (_V, [_P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _P]),
+    "nvte_amd_moe_forward_workspace_size": (_SZ, [_SZ] * 5),
+    "nvte_amd_moe_forward": (_V, [_P] * 8 + [_SZ] * 5 + [_I, _I, _P, _SZ, _P]),
     # transformer_engine.h
     "nvte_create_tensor": (_P, [_I]),
     "nvte_create_tensors": (_V, [_I, C.POINTER(_P), _SZ]),

@@ -26,7 +26,8 @@ from .tensor import (DType, Float8CurrentScalingQuantizer, Float8Quantizer, Floa
 __all__ = ["multi_tensor_applier", "multi_tensor_scale", "multi_tensor_compute_scale_and_scale_inv",
            "multi_tensor_compute_scale_inv_e8m0", "multi_tensor_adam_fp8",
            "mxfp8_scaling_compute_partial_amax", "mxfp8_scaling_partial_cast",
-           "quantize_master_weights", "cast_master_weights_to_fp8", "post_all_gather_processing"]
+           "quantize_master_weights", "cast_master_weights_to_fp8", "post_all_gather_processing",
+           "grad_norm", "clip_grad_norm"]
 
 
 # =====================================================================================
@@ -119,6 +120,101 @@ class MultiTensorApply:
 
 
 multi_tensor_applier = MultiTensorApply(2048 * 32)
+
+
+# =====================================================================================
+# global gradient norm and clipping
+# =====================================================================================
+_GRAD_DTYPES = {torch.float32: int(DType.kFloat32), torch.float16: int(DType.kFloat16), torch.bfloat16: int(DType.kBFloat16)}
+
+
+class _Arrays:
+    """Host arrays of addresses, element counts and dtypes for the list entry points of amd_ext.h."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor], name: str):
+        n = len(tensors)
+        self.n, self.device = n, tensors[0].device if n else torch.device("cuda", torch.cuda.current_device())
+        for i, t in enumerate(tensors):
+            if not t.is_cuda:
+                raise RuntimeError(f"{name}[{i}] is on {t.device}: gradients are clipped on the GPU only (no CPU fallback in this "
+                                   "library)")
+            if t.device != self.device:
+                raise ValueError(f"{name}[{i}] is on {t.device}, but {name}[0] is on {self.device}")
+            if t.dtype not in _GRAD_DTYPES:
+                raise TypeError(f"{name}[{i}] must be float32, float16 or bfloat16, got {t.dtype}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name}[{i}] must be contiguous")
+        self.ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in tensors])
+        self.numels = (C.c_size_t * n)(*[t.numel() for t in tensors])
+        self.dtypes = (C.c_int * n)(*[_GRAD_DTYPES[t.dtype] for t in tensors])
+
+
+def _all_reduce_sum(t: torch.Tensor, group):
+    import torch.distributed as dist
+    if dist.get_backend(group) == "gloo" and t.is_cuda:
+        h = t.cpu()
+        dist.all_reduce(h, group=group)
+        t.copy_(h)
+    else:
+        dist.all_reduce(t, group=group)
+
+
+def grad_norm(grads: Sequence[torch.Tensor], group=None) -> torch.Tensor:
+    """2-norm of all elements of all ``grads`` together, fp32 [1] on their device (nothing is read on the host).
+
+    The tensors are contiguous and fp32, fp16 or bf16, mixed at will; squares are summed in 64 bits in a fixed order.  With a
+    process ``group`` the ranks' sums of squares are added first (every rank passes the gradients only it holds)."""
+    return _grad_norm(list(grads), group)[1]
+
+
+def _grad_norm(grads, group):
+    arr = _Arrays(grads, "grads")
+    with torch.cuda.device(arr.device):
+        norm = torch.empty(1, dtype=torch.float32, device=arr.device)
+        total = torch.empty(1, dtype=torch.float64, device=arr.device)
+        size = api.nvte_amd_grad_norm_workspace_size(arr.numels, arr.n)
+        ws = torch.empty(size, dtype=torch.uint8, device=arr.device)
+        api.nvte_amd_grad_norm(arr.ptrs, arr.numels, arr.dtypes, arr.n, total.data_ptr(), norm.data_ptr(), ws.data_ptr(), size,
+                               current_stream_ptr())
+        if group is not None:
+            _all_reduce_sum(total, group)
+            norm = total.sqrt().to(torch.float32)
+    return total, norm, arr
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, outs: Optional[Sequence[torch.Tensor]] = None,
+                   eps: float = 1e-6, group=None) -> torch.Tensor:
+    """``outs[i] = grads[i] * min(1, max_norm / (norm + eps))`` with ``norm = grad_norm(grads, group)``, which is returned.
+
+    ``outs`` defaults to ``grads`` (in place); it may hold other tensors of the same lengths and of any of the three dtypes, for
+    instance the fp32 gradients that ``multi_tensor_adam_fp8`` reads.  An output may be its own gradient and overlap nothing else,
+    so in place no tensor may be listed twice.  An Inf or NaN gradient makes the norm Inf or NaN (the factor 0 or NaN): the norm
+    says whether to skip the step, as ``multi_tensor_scale``'s flag does."""
+    grads = list(grads)
+    outs = grads if outs is None else list(outs)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(grads)} gradients, but {len(outs)} outputs")
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if g is not o and g.numel() != o.numel():
+            raise ValueError(f"grads[{i}] has {g.numel()} elements, but outs[{i}] has {o.numel()}")
+    if group is not None:
+        total, norm, arr = _grad_norm(grads, group)
+    else:
+        arr = _Arrays(grads, "grads")
+    out = arr if outs is grads else _Arrays(outs, "outs")
+    if arr.device != out.device:
+        raise ValueError(f"grads are on {arr.device}, but outs are on {out.device}")
+    with torch.cuda.device(arr.device):
+        if group is not None:
+            api.nvte_amd_clip_by_sum_of_squares(arr.ptrs, out.ptrs, arr.numels, arr.dtypes, out.dtypes, arr.n, total.data_ptr(),
+                                                C.c_float(max_norm), C.c_float(eps), norm.data_ptr(), current_stream_ptr())
+            return norm
+        norm = torch.empty(1, dtype=torch.float32, device=arr.device)
+        size = api.nvte_amd_grad_norm_workspace_size(arr.numels, arr.n)
+        ws = torch.empty(size, dtype=torch.uint8, device=arr.device)
+        api.nvte_amd_clip_grad_norm(arr.ptrs, out.ptrs, arr.numels, arr.dtypes, out.dtypes, arr.n, C.c_float(max_norm),
+                                    C.c_float(eps), norm.data_ptr(), ws.data_ptr(), size, current_stream_ptr())
+    return norm
 
 
 # =====================================================================================
