@@ -4,15 +4,17 @@
 //   u[t] = B_a^T dy[t]                   dx[t] = base_grad[t] + s_a A_a^T u[t]
 //   dA_a = sum_t s_a u[t] (x) x[t]       dB_a  = sum_t dy[t] (x) s_a v[t]             sums over the tokens of adapter a
 //
-// Four kernels: `shrink` (activations to rank vectors), `expand` (rank vectors to activations), `wgrad` (outer products summed
-// over an adapter's tokens) and its `join`; `plan` lists the tokens of every adapter for the last two.  All of them are bound by
-// the activations they stream (2 T (K + O) bytes and more against 2 T r (K + O) operations, r <= 128); the pools stay in L2.
-// A tile of tokens walks the distinct adapters among its own tokens, so any order of ids is right; values of other
-// adapters' rows are never added, only selected, so a NaN or Inf stays in its own rows.
+// Forward: `shrink` (activations to rank vectors), then `expand` (rank vectors to activations).  Backward: `prepare` (the tokens
+// of every adapter; B transposed, so that `shrink` reads it like A), `shrink`, `expand` together with `pack` (rank vectors as matrix
+// operands, in the tokens' order), `wgrad` (outer products summed over an adapter's tokens), `join`.
+// All of them are bound by the activations they stream (2 T (K + O) bytes and more against 2 T r (K + O) operations, r <= 128);
+// the pools stay in L2.  A tile of tokens walks the distinct adapters among its own tokens, so any order of ids is right;
+// values of other adapters' rows are never added, only selected, so a NaN or Inf stays in its own rows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.h"
 #include "device_utils.h"
@@ -32,8 +34,7 @@ __device__ __forceinline__ int valid_id(const int *ids, int64_t t, int64_t token
 }
 
 // ====================================================================================
-// shrink: out[slice][t][j] = sum over the slice's k of in[t][k] * w(j, k)
-// w(j, k) = pool[a][j][k], or pool[a][k][j] (KMAJOR)
+// shrink: out[slice][t][j] = sum over the slice's k of in[t][k] * pool[a][j][k]
 // ====================================================================================
 struct ShrinkArgs {
   const uint16_t *in, *pool;
@@ -43,53 +44,47 @@ struct ShrinkArgs {
   int features, rank, num, slice;
 };
 
-template <typename E, int RT, int MT, int NW, bool VEC, bool KMAJOR>
-__device__ __forceinline__ void shrink_sum(const ShrinkArgs &p, const uint16_t *const (&row)[MT], const uint16_t *w, int wave,
-                                           int lane, int begin, int end, f32x4 (&acc)[MT][RT]) {
-  const int kg = (lane >> 4) * 8;
-  // NW * 64 elements of k per turn; a wave's two steps of 32 are one 128-byte line of every row
-  for (int k0 = begin + wave * 64; k0 < end; k0 += NW * 64) {
-    u32x4 a[2][MT], b[2][RT];
+template <int MT, int RT, bool GUARD>
+struct ShrinkBlock {  // 64 k of every row: one 128-byte line, two operands
+  u32x4 a[MT][2], b[RT][2];
+  __device__ __forceinline__ void load(const uint16_t *const (&row)[MT], const uint16_t *const (&w)[RT], int k, int end) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int k = k0 + 32 * h + kg;
-      // what lies behind the slice belongs to the next one; `end` is a multiple of 64 or the row's end
 #pragma unroll
-      for (int m = 0; m < MT; ++m) a[h][m] = row8<VEC>(row[m], k, end);
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (GUARD) a[m][h] = load8_head(row[m] + k + 32 * h, end - k - 32 * h);
+        else a[m][h] = load8(row[m] + k + 32 * h);
+      }
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        const int col = min(j * 16 + (lane & 15), p.rank - 1);  // columns from `rank` on are computed and not kept
-        if constexpr (KMAJOR) {
-          u32x4 v = {0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (k + i < end) v[i >> 1] |= static_cast<uint32_t>(w[static_cast<int64_t>(k + i) * p.rank + col]) << (16 * (i & 1));
-          b[h][j] = v;
-        } else {
-          b[h][j] = row8<VEC>(w + static_cast<int64_t>(col) * p.features, k, end);
-        }
+        if constexpr (GUARD) b[j][h] = load8_head(w[j] + k + 32 * h, end - k - 32 * h);
+        else b[j][h] = load8(w[j] + k + 32 * h);
       }
     }
+  }
+  template <typename E>
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[MT][RT]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[m][j] = mfma16<E>(a[h][m], b[h][j], acc[m][j]);
+        for (int j = 0; j < RT; ++j) acc[m][j] = mfma16<E>(a[m][h], b[j][h], acc[m][j]);
   }
-}
+};
 
-// grid: token tiles x slices x phases (the tile's n-th distinct adapter is phase n % gridDim.z's)
-template <typename E, int RT, int MT, int NW, bool KMAJOR>
-__global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p, bool vec) {
-  __shared__ float red[NW][MT * RT * 256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// grid: token tiles x slices x phases (the tile's n-th distinct adapter is phase n % gridDim.z's); the NW waves share the slice
+template <typename E, int RT, int MT, int NW, int U>
+__global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
+  __shared__ f32x4 red[NW][MT * RT][64];
+  const int lane = threadIdx.x & 63, wave = wave_index();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
   const int id = lane < 16 * MT ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
   const uint16_t *row[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) row[m] = p.in + min(t0 + m * 16 + (lane & 15), p.tokens - 1) * p.features;
   const int begin = blockIdx.y * p.slice, end = min(begin + p.slice, p.features);
+  const int first = begin + wave * 64, kg = 8 * (lane >> 4);
 
   unsigned phase = 0;
   for (uint64_t left = __ballot(id >= 0); left != 0;) {
@@ -98,26 +93,63 @@ __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p, bool vec)
     left &= ~mine;
     if (phase++ % gridDim.z != blockIdx.z) continue;
     f32x4 acc[MT][RT] = {};
-    const uint16_t *w = p.pool + static_cast<int64_t>(cur) * p.rank * p.features;
-    if (vec) shrink_sum<E, RT, MT, NW, true, KMAJOR>(p, row, w, wave, lane, begin, end, acc);
-    else shrink_sum<E, RT, MT, NW, false, KMAJOR>(p, row, w, wave, lane, begin, end, acc);
+    const uint16_t *w[RT];  // rank rows from `rank` on are computed from the last one and not kept
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+      w[j] = p.pool + (static_cast<int64_t>(cur) * p.rank + min(j * 16 + (lane & 15), p.rank - 1)) * p.features;
+    int k = first;
+    for (; k + NW * 64 * (U - 1) + 64 <= end; k += NW * 64 * U) {
+      ShrinkBlock<MT, RT, false> block[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) block[u].load(row, w, k + u * NW * 64 + kg, end);
+      __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first product waits for one
+#pragma unroll
+      for (int u = 0; u < U; ++u) block[u].template multiply<E>(acc);
+    }
+    if constexpr (U > 1) {
+      for (; k + 64 <= end; k += NW * 64) {
+        ShrinkBlock<MT, RT, false> block;
+        block.load(row, w, k + kg, end);
+        block.template multiply<E>(acc);
+      }
+    }
+    if (k < end) {
+      ShrinkBlock<MT, RT, true> block;
+      block.load(row, w, k + kg, end);
+      block.template multiply<E>(acc);
+    }
+    __syncthreads();  // the last adapter's sums are read
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int j = 0; j < RT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][((m * RT + j) * 4 + i) * 64 + lane] = acc[m][j][i];
+      for (int j = 0; j < RT; ++j) red[wave][m * RT + j][lane] = acc[m][j];
     __syncthreads();
-    for (int e = threadIdx.x; e < MT * RT * 256; e += NW * 64) {
-      const int l = e & 63, i = (e >> 6) & 3, j = (e >> 8) % RT, m = (e >> 8) / RT;
-      const int tok = m * 16 + (l >> 4) * 4 + i, col = j * 16 + (l & 15);
-      float s = 0.f;
+    for (int e = threadIdx.x; e < MT * RT * 64; e += NW * 64) {
+      const int l = e & 63, j = (e >> 6) % RT, m = (e >> 6) / RT;
+      f32x4 s = red[0][m * RT + j][l];
 #pragma unroll
-      for (int n = 0; n < NW; ++n) s += red[n][e];
-      if (((mine >> tok) & 1) && col < p.rank) p.out[(blockIdx.y * p.tokens + t0 + tok) * p.rank + col] = s;
+      for (int n = 1; n < NW; ++n) s += red[n][m * RT + j][l];
+      const int col = j * 16 + (l & 15);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = m * 16 + (l >> 4) * 4 + i;
+        if (((mine >> tok) & 1) && col < p.rank) p.out[(blockIdx.y * p.tokens + t0 + tok) * p.rank + col] = s[i];
+      }
     }
-    __syncthreads();
   }
+}
+
+// one value of a rank vector: its slices in order, eight at a time on their way
+__device__ __forceinline__ float sum_slices(const float *p, int slices, int64_t stride) {
+  float s = 0.f;
+  for (int s0 = 0; s0 < slices; s0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s0 + i < slices ? p[(s0 + i) * stride] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
+  }
+  return s;
 }
 
 // ====================================================================================
@@ -134,95 +166,35 @@ struct ExpandArgs {
   int slices, features, rank, num, cols;  // cols: columns per workgroup, a multiple of 512
 };
 
-// the eight operands of columns c0 + 8 m + f (m = lane % 16): one per f, eight ranks j0 + 8 (lane / 16) of each
-template <bool VEC, bool RMAJOR>
-__device__ __forceinline__ void pool_block(const uint16_t *w, int lane, int c0, int j0, int features, int rank, u32x4 (&f)[8]) {
-  const int c = c0 + 8 * (lane & 15), j = j0 + 8 * (lane >> 4);
+// A wave's step is 128 columns: operand f holds columns c0 + place(m) + f of its rows m = 0 .. 15.  D then leaves a lane (token n,
+// lane group q, register i) with the eight neighbours c0 + 32 i + 8 q + 0 .. 7 over f, so that each of the four stores of a step writes 64
+// contiguous bytes of every token.
+__device__ __forceinline__ int place(int m) { return 32 * (m & 3) + 8 * (m >> 2); }
+
+template <bool RMAJOR>
+__device__ __forceinline__ void pool_block(const ExpandArgs &p, int adapter, int lane, int c0, int j0, u32x4 (&f)[8]) {
+  const int c = c0 + place(lane & 15), j = j0 + 8 * (lane >> 4);
+  const uint16_t *w = p.pool + static_cast<int64_t>(adapter) * p.rank * p.features;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
   if constexpr (RMAJOR) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = j + i < rank ? row8<VEC>(w + static_cast<int64_t>(j + i) * features, c, features) : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < 8; ++i) f[i] = j + i < p.rank ? load8_head(w + static_cast<int64_t>(j + i) * p.features + c, p.features - c) : zero;
     transpose8x8(f);
   } else {
+    const uint16_t *end = p.pool + static_cast<int64_t>(p.num) * p.rank * p.features;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = c + i < features ? row8<VEC>(w + static_cast<int64_t>(c + i) * rank, j, rank) : u32x4{0u, 0u, 0u, 0u};
-  }
-}
-
-template <typename E>
-__device__ __forceinline__ void store_row8(const ExpandArgs &p, int64_t t, int c, bool vec, const float (&add)[8]) {
-  const int64_t at = t * p.features + c;
-  if (vec) {
-    if (c >= p.features) return;
-    float b[8] = {};
-    if (p.base != nullptr) Raw8<E>::load_cached(reinterpret_cast<const E *>(p.base) + at).widen8(b);
-    E o[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) narrow(b[k] + add[k], o[k]);
-    *reinterpret_cast<u32x4 *>(p.out + at) = *reinterpret_cast<const u32x4 *>(o);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (c + k >= p.features) return;
-      const float b = p.base != nullptr ? widen(reinterpret_cast<const E *>(p.base)[at + k]) : 0.f;
-      narrow(b + add[k], reinterpret_cast<E *>(p.out)[at + k]);
+    for (int i = 0; i < 8; ++i) {
+      const int valid = c + i < p.features ? p.rank - j : 0;
+      f[i] = valid > 0 ? load8_head(w + static_cast<int64_t>(c + i) * p.rank + j, valid, end) : zero;
     }
   }
 }
 
-template <typename E, int KT, int MT, bool VEC, bool RMAJOR>
-__device__ __forceinline__ void expand_columns(const ExpandArgs &p, bool vec_rows, int64_t t0, int id, uint64_t tokens_used,
-                                               const u32x4 (&hi)[MT][KT], const u32x4 (&lo)[MT][KT], int wave, int lane) {
-  const int begin = blockIdx.y * p.cols, end = min(begin + p.cols, p.features);
-  int my_id[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) my_id[m] = __shfl(id, m * 16 + (lane & 15), 64);
-  for (int c0 = begin + wave * 128; c0 < end; c0 += 512) {
-    f32x4 res[MT][8] = {};
-    for (uint64_t left = tokens_used; left != 0;) {
-      const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-      left &= ~__ballot(id == cur);
-      const uint16_t *w = p.pool + static_cast<int64_t>(cur) * p.rank * p.features;
-      f32x4 acc[MT][8] = {};
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        u32x4 f[8];
-        pool_block<VEC, RMAJOR>(w, lane, c0, k * 32, p.features, p.rank, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const Terms<E> terms(f[i]);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m][i] = mfma16_split<E>(terms, hi[m][k], lo[m][k], acc[m][i]);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) res[m][i] = my_id[m] == cur ? acc[m][i] : res[m][i];
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t t = t0 + m * 16 + (lane & 15);
-      if (t >= p.tokens) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float add[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) add[k] = res[m][k][i];
-        store_row8<E>(p, t, c0 + 8 * (4 * (lane >> 4) + i), vec_rows, add);
-      }
-    }
-  }
-}
-
-// grid: token tiles x column ranges
 template <typename E, int KT, int MT, bool RMAJOR>
-__global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p, bool vec_pool, bool vec_rows) {
-  constexpr int kRow = KT * 32 + 8;  // 16-byte aligned rows, neighbouring rows in different banks
-  __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][kRow], s_lo[16 * MT][kRow];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
+__device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, int columns, uint16_t (*s_hi)[KT * 32 + 8],
+                                            uint16_t (*s_lo)[KT * 32 + 8]) {
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const int64_t t0 = tile * (16 * MT);
   const int id = lane < 16 * MT ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
   const uint64_t used = __ballot(id >= 0);
   if (used == 0 && p.base == p.out) return;
@@ -230,8 +202,8 @@ __global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p, bool vec_pool
     const int tok = e / (KT * 32), j = e % (KT * 32);
     float v = 0.f;
     if (((used >> tok) & 1) && j < p.rank) {
-      for (int s = 0; s < p.slices; ++s) v += p.low[(s * p.tokens + t0 + tok) * p.rank + j];
-      if (p.scaling != nullptr) v *= p.scaling[p.ids[t0 + tok]];
+      const float s = p.scaling != nullptr ? p.scaling[p.ids[t0 + tok]] : 1.f;
+      v = s * sum_slices(p.low + (t0 + tok) * p.rank + j, p.slices, p.tokens * p.rank);
     }
     __bf16 h, l;
     split1(v, h, l);
@@ -240,166 +212,322 @@ __global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p, bool vec_pool
   }
   __syncthreads();
   u32x4 hi[MT][KT], lo[MT][KT];
+  int my_id[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    my_id[m] = __shfl(id, m * 16 + (lane & 15), 64);
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
       hi[m][k] = *reinterpret_cast<const u32x4 *>(&s_hi[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
       lo[m][k] = *reinterpret_cast<const u32x4 *>(&s_lo[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
     }
-  if (vec_pool) expand_columns<E, KT, MT, true, RMAJOR>(p, vec_rows, t0, id, used, hi, lo, wave, lane);
-  else expand_columns<E, KT, MT, false, RMAJOR>(p, vec_rows, t0, id, used, hi, lo, wave, lane);
+  }
+  const int begin = columns * p.cols, end = min(begin + p.cols, p.features);
+  for (int c0 = begin + wave * 128; c0 < end; c0 += 512) {
+    // the columns' old values travel while the products run
+    u32x4 base[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t t = t0 + m * 16 + (lane & 15);
+        const int c = c0 + 32 * i + 8 * (lane >> 4);
+        base[m][i] = u32x4{0u, 0u, 0u, 0u};
+        if (p.base != nullptr && t < p.tokens) base[m][i] = load8_head(p.base + t * p.features + c, p.features - c);
+      }
+    f32x4 res[MT][8] = {};
+    for (uint64_t left = used; left != 0;) {
+      const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+      left &= ~__ballot(id == cur);
+      u32x4 f[KT][8];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) pool_block<RMAJOR>(p, cur, lane, c0, k * 32, f[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f32x4 acc[MT] = {};
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          const Terms<E> terms(f[k][i]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] = mfma16_split<E>(terms, hi[m][k], lo[m][k], acc[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) res[m][i] = my_id[m] == cur ? acc[m] : res[m][i];
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t t = t0 + m * 16 + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 32 * i + 8 * (lane >> 4);
+        E o[8];
+        const E *old = reinterpret_cast<const E *>(&base[m][i]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) narrow(widen(old[k]) + res[m][k][i], o[k]);
+        uint16_t *to = p.out + t * p.features + c;
+        if (t < p.tokens && c + 8 <= p.features) {
+          store8(to, *reinterpret_cast<const u32x4 *>(o));
+        } else if (t < p.tokens) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (c + k < p.features) reinterpret_cast<E *>(to)[k] = o[k];
+        }
+      }
+    }
+  }
+}
+
+// grid: token tiles x column ranges
+template <typename E, int KT, int MT, bool RMAJOR>
+__global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p) {
+  // 16-byte aligned rows, neighbouring rows in different banks
+  __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
+  expand_tile<E, KT, MT, RMAJOR>(p, blockIdx.x, blockIdx.y, s_hi, s_lo);
 }
 
 // ====================================================================================
-// plan: the tokens of every adapter in rising order, and how many work items of `per_item` tokens it has
-// one workgroup per adapter; every one counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged
+// prepare: the tokens of every adapter in rising order, each adapter's list padded to whole blocks of 32 with -1; where they
+// begin; where its work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to [rank][features].
+// One workgroup per adapter counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged; its sixteen waves own
+// consecutive stretches of the tokens.
 // ====================================================================================
+constexpr int kBlock = 32;
+
 struct Plan {
-  int *order;       // [tokens]
-  int *token_base;  // [num + 1] first entry of every adapter in `order`
+  int *order;       // [most_blocks * 32]
+  int *block_base;  // [num + 1] first block of every adapter in `order`
   int *item_base;   // [num + 1] first work item of every adapter
 };
+struct PrepareArgs {
+  const int *ids;
+  const uint16_t *pool;  // null: no transpose
+  uint16_t *transposed;
+  Plan plan;             // order null: no lists
+  int64_t tokens;
+  int features, rank, num, per_item, lists;  // lists: workgroups of the first part
+};
 
-__device__ __forceinline__ int block_sum_int(int v, int *scratch) {  // 256 threads, valid in every thread
+__device__ __forceinline__ int sum_1024(int v, int *scratch) {  // valid in every thread
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
-  const int s = scratch[0] + scratch[1] + scratch[2] + scratch[3];
-  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += scratch[w];
   return s;
 }
 
-__global__ __launch_bounds__(256) void plan_kernel(const int *ids, int64_t tokens, int num, int per_item, Plan out) {
-  __shared__ int hist[kMaxAdapters];
-  __shared__ int scratch[4];
-  const int a = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = threadIdx.x; i < num; i += 256) hist[i] = 0;
+__device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t stretch = ((p.tokens + 15) / 16 + 63) / 64 * 64, from = wave * stretch;
+  const int64_t to = min(from + stretch, p.tokens);
+  for (int i = threadIdx.x; i < p.num; i += 1024) hist[i] = 0;
   __syncthreads();
-  for (int64_t t = threadIdx.x; t < tokens; t += 256) {
-    const int id = valid_id(ids, t, tokens, num);
-    if (id >= 0) atomicAdd(&hist[id], 1);
-  }
-  __syncthreads();
-  int before = 0, items = 0;
-  for (int i = threadIdx.x; i < a; i += 256) {
-    before += hist[i];
-    items += (hist[i] + per_item - 1) / per_item;
-  }
-  before = block_sum_int(before, scratch);
-  items = block_sum_int(items, scratch);
-  const int mine = hist[a];
-  if (threadIdx.x == 0) {
-    out.token_base[a] = before;
-    out.item_base[a] = items;
-    if (a == num - 1) {
-      out.token_base[num] = before + mine;
-      out.item_base[num] = items + (mine + per_item - 1) / per_item;
+  for (int64_t t0 = from; t0 < to; t0 += 64) {
+    const int id = t0 + lane < to ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
+    for (uint64_t left = __ballot(id >= 0); left != 0;) {  // one addition per distinct id: a run would queue up on one address
+      const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+      const uint64_t same = __ballot(id == cur);
+      left &= ~same;
+      if (lane == 0) atomicAdd(&hist[cur], __popcll(same));
     }
   }
-  int at = before;
-  const int stop = before + mine;
-  for (int64_t t0 = 0; t0 < tokens && at < stop; t0 += 256) {
-    const int64_t t = t0 + threadIdx.x;
-    const bool hit = valid_id(ids, t, tokens, num) == a;
-    const uint64_t m = __ballot(hit);
-    if (lane == 0) scratch[wave] = __popcll(m);
-    __syncthreads();
-    int off = at;
-    for (int w = 0; w < wave; ++w) off += scratch[w];
-    if (hit) out.order[off + __popcll(m & ((1ull << lane) - 1))] = static_cast<int>(t);
-    at += scratch[0] + scratch[1] + scratch[2] + scratch[3];
-    __syncthreads();
+  __syncthreads();
+  int blocks = 0, items = 0;
+  for (int i = threadIdx.x; i < a; i += 1024) {
+    const int b = (hist[i] + kBlock - 1) / kBlock;
+    blocks += b;
+    items += (b + p.per_item - 1) / p.per_item;
   }
+  blocks = sum_1024(blocks, scratch);
+  items = sum_1024(items, scratch);
+  const int mine = hist[a], my_blocks = (mine + kBlock - 1) / kBlock;
+  if (threadIdx.x == 0) {
+    p.plan.block_base[a] = blocks;
+    p.plan.item_base[a] = items;
+    if (a == p.num - 1) {
+      p.plan.block_base[p.num] = blocks + my_blocks;
+      p.plan.item_base[p.num] = items + (my_blocks + p.per_item - 1) / p.per_item;
+    }
+  }
+  if (mine == 0) return;
+  int *order = p.plan.order + static_cast<int64_t>(blocks) * kBlock;
+  int count = 0;
+  for (int64_t t0 = from; t0 < to; t0 += 64)
+    count += __popcll(__ballot(t0 + lane < to && p.ids[t0 + lane] == a));
+  __syncthreads();
+  if (lane == 0) scratch[wave] = count;
+  __syncthreads();
+  int at = 0;
+  for (int w = 0; w < wave; ++w) at += scratch[w];
+  for (int64_t t0 = from; t0 < to; t0 += 64) {
+    const bool hit = t0 + lane < to && p.ids[t0 + lane] == a;
+    const uint64_t m = __ballot(hit);
+    if (hit) order[at + __popcll(m & ((1ull << lane) - 1))] = static_cast<int>(t0) + lane;
+    at += __popcll(m);
+  }
+  if (threadIdx.x < my_blocks * kBlock - mine) order[mine + threadIdx.x] = -1;
+}
+
+// 64 features of one adapter's matrix
+__device__ void transpose_rows(const PrepareArgs &p, int64_t piece, uint16_t *s) {
+  const int per_adapter = (p.features + 63) / 64;
+  const int64_t a = piece / per_adapter;
+  const int f0 = static_cast<int>(piece % per_adapter) * 64, n = min(64, p.features - f0);
+  const uint16_t *in = p.pool + (a * p.features + f0) * p.rank;
+  for (int e = threadIdx.x; e < n * p.rank; e += 1024) s[e / p.rank * (p.rank + 1) + e % p.rank] = in[e];
+  __syncthreads();
+  uint16_t *out = p.transposed + a * p.features * p.rank + f0;
+  for (int e = threadIdx.x; e < 64 * p.rank; e += 1024) {
+    const int f = e & 63, j = e >> 6;
+    if (f < n) out[static_cast<int64_t>(j) * p.features + f] = s[f * (p.rank + 1) + j];
+  }
+}
+
+__global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
+  __shared__ union {
+    int hist[kMaxAdapters];
+    uint16_t rows[64 * (kMaxRank + 1)];
+  } s;
+  __shared__ int scratch[16];
+  if (static_cast<int>(blockIdx.x) < p.lists) list_tokens(p, blockIdx.x, s.hist, scratch);
+  else transpose_rows(p, blockIdx.x - p.lists, s.rows);
+}
+
+// ====================================================================================
+// pack: the scaled rank vectors of every block of 32 tokens as matrix operands: [block][16 ranks][hi, lo][lane][8 tokens]
+// ====================================================================================
+struct PackSide {
+  const float *low;  // [slices][tokens][rank]
+  uint16_t *packed;
+  int slices;
+};
+struct PackArgs {
+  PackSide side[2];
+  const float *scaling;
+  Plan plan;
+  int64_t tokens;
+  int rank, num;
+};
+
+// the adapter whose range of `base` holds `i` (adapters without tokens have none)
+__device__ __forceinline__ int owner_of(const int *base, int num, int i) {
+  int a = 0;
+  for (int hi = num; hi - a > 1;) {
+    const int mid = (a + hi) >> 1;
+    if (base[mid] <= i) a = mid; else hi = mid;
+  }
+  return a;
+}
+
+__device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &side, int block) {
+  if (block >= p.plan.block_base[p.num]) return;
+  const float scale = p.scaling != nullptr ? p.scaling[owner_of(p.plan.block_base, p.num, block)] : 1.f;
+  const int tiles = (p.rank + 15) / 16;
+  uint16_t *out = side.packed + static_cast<int64_t>(block) * tiles * 1024;
+  // neighbouring threads take neighbouring ranks of one token
+  for (int e = threadIdx.x; e < kBlock * tiles * 16; e += 256) {
+    const int j = e % (tiles * 16), tok = e / (tiles * 16);
+    const int t = p.plan.order[block * kBlock + tok];
+    float v = 0.f;
+    if (t >= 0 && j < p.rank) v = scale * sum_slices(side.low + static_cast<int64_t>(t) * p.rank + j, side.slices, p.tokens * p.rank);
+    __bf16 h, l;
+    split1(v, h, l);
+    const int at = (j >> 4) * 1024 + ((j & 15) + 16 * (tok >> 3)) * 8 + (tok & 7);
+    out[at] = bits16(h);
+    out[at + 512] = bits16(l);
+  }
+}
+
+// the backward pass's `expand` and `pack` read the same rank vectors and nothing of each other: one launch
+template <typename E, int KT, int MT>
+__global__ __launch_bounds__(256) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int blocks) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
+  const int b = blockIdx.x;
+  if (b < 2 * blocks) pack_block(q, b < blocks ? q.side[0] : q.side[1], b < blocks ? b : b - blocks);
+  else expand_tile<E, KT, MT, true>(p, (b - 2 * blocks) % tiles, (b - 2 * blocks) / tiles, s_hi, s_lo);
 }
 
 // ====================================================================================
 // wgrad: one work item's dA [r][K] = sum_t w[t] (x) x[t] and dB [O][r] = sum_t dy[t] (x) w[t]
 // ====================================================================================
 struct WgradSide {
-  const uint16_t *z;  // activations [tokens][features]
-  const float *low;   // rank vectors [slices][tokens][rank]
-  void *grad;         // [num][rank][features] or [num][features][rank]
-  float *part;        // per item, the same layout in fp32
-  int slices, features, groups;  // groups: workgroups along the features, 512 columns each
-  bool vec;
+  const uint16_t *z;       // activations [tokens][features]
+  const uint16_t *packed;  // rank vectors
+  void *grad;              // [num][rank][features] or [num][features][rank]
+  float *part;             // per item, the same layout in fp32
+  int features, groups;    // groups: workgroups along the features, 512 columns each
 };
 struct WgradArgs {
   WgradSide a, b;
-  const float *scaling;
   Plan plan;
-  int64_t tokens;
   int rank, num, per_item, grad_type;
 };
 
-constexpr int kStep = 64;  // tokens whose rank vectors are staged at a time
+template <typename E, int RT>
+struct WgradBlock {  // 32 tokens x 128 columns, and their rank vectors
+  u32x4 z[8], w[RT][2];
+  __device__ __forceinline__ void load(const WgradSide &side, const int *order, int64_t block, int rank_tiles, int j0, int c, int lane) {
+    const int *tokens = order + block * kBlock + 8 * (lane >> 4);
+    const uint16_t *w0 = side.packed + (block * rank_tiles + j0) * 1024 + lane * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = tokens[i];
+      z[i] = u32x4{0u, 0u, 0u, 0u};
+      if (t >= 0) z[i] = load8_head(side.z + static_cast<int64_t>(t) * side.features + c, side.features - c);
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      w[j][0] = *reinterpret_cast<const u32x4 *>(w0 + min(j, rank_tiles - j0 - 1) * 1024);
+      w[j][1] = *reinterpret_cast<const u32x4 *>(w0 + min(j, rank_tiles - j0 - 1) * 1024 + 512);
+    }
+  }
+  template <bool IS_B>
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[RT][8]) {
+    transpose8x8(z);
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+      const Terms<E> terms(z[f]);
+#pragma unroll
+      for (int j = 0; j < RT; ++j) acc[j][f] = mfma16_split<E, !IS_B>(terms, w[j][0], w[j][1], acc[j][f]);
+    }
+  }
+};
 
-template <typename E, int RT, bool VEC, bool IS_B>
-__device__ __forceinline__ void wgrad_side(const WgradArgs &p, const WgradSide &side, int group, uint16_t (*s_hi)[RT][512],
-                           uint16_t (*s_lo)[RT][512]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename E, int RT, bool IS_B>
+__device__ __forceinline__ void wgrad_side(const WgradArgs &p, const WgradSide &side, int group) {
+  const int lane = threadIdx.x & 63, wave = wave_index();
   const int item = blockIdx.y;
   if (item >= p.plan.item_base[p.num]) return;
-  int a = 0;
-  for (int hi = p.num; hi - a > 1;) {  // the adapter whose items hold this one (adapters without tokens have none)
-    const int mid = (a + hi) >> 1;
-    if (p.plan.item_base[mid] <= item) a = mid; else hi = mid;
-  }
-  const int first = p.plan.token_base[a] + (item - p.plan.item_base[a]) * p.per_item;
-  const int last = min(first + p.per_item, p.plan.token_base[a + 1]);
+  const int a = __builtin_amdgcn_readfirstlane(owner_of(p.plan.item_base, p.num, item));
+  const int first = __builtin_amdgcn_readfirstlane(p.plan.block_base[a] + (item - p.plan.item_base[a]) * p.per_item);
+  const int last = __builtin_amdgcn_readfirstlane(min(first + p.per_item, p.plan.block_base[a + 1]));
   const bool whole = p.plan.item_base[a + 1] - p.plan.item_base[a] == 1;
-  const float scale = p.scaling != nullptr ? p.scaling[a] : 1.f;
   const int c0 = group * 512 + wave * 128, c = c0 + 8 * (lane & 15);
-  const int j0 = blockIdx.z * 64, ranks = min(p.rank - j0, 64);
+  if (c0 >= side.features) return;
+  const int rank_tiles = (p.rank + 15) / 16, j0 = blockIdx.z * 4;
   f32x4 acc[RT][8] = {};
-  for (int s0 = first; s0 < last; s0 += kStep) {
-    u32x4 z[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = s0 + h * 32 + (lane >> 4) * 8 + i;
-        z[h][i] = at < last ? row8<VEC>(side.z + static_cast<int64_t>(p.plan.order[at]) * side.features, c, side.features)
-                            : u32x4{0u, 0u, 0u, 0u};
-      }
-    __syncthreads();  // the last step's operands are read
-    for (int e = threadIdx.x; e < kStep * RT * 16; e += 256) {
-      const int tok = e / (RT * 16), j = e % (RT * 16), at = s0 + tok;
-      float v = 0.f;
-      if (at < last && j < ranks) {
-        const int64_t t = p.plan.order[at];
-        for (int s = 0; s < side.slices; ++s) v += side.low[(s * p.tokens + t) * p.rank + j0 + j];
-        v *= scale;
-      }
-      __bf16 h, l;
-      split1(v, h, l);
-      const int slot = (j & 15) * 8 + ((tok >> 3) & 3) * 128 + (tok & 7);  // operand order: lane, then eight tokens
-      s_hi[tok >> 5][j >> 4][slot] = bits16(h);
-      s_lo[tok >> 5][j >> 4][slot] = bits16(l);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      transpose8x8(z[h]);
-      u32x4 wh[RT], wl[RT];
-#pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        wh[j] = *reinterpret_cast<const u32x4 *>(&s_hi[h][j][lane * 8]);
-        wl[j] = *reinterpret_cast<const u32x4 *>(&s_lo[h][j][lane * 8]);
-      }
-#pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        const Terms<E> terms(z[h][f]);
-#pragma unroll
-        for (int j = 0; j < RT; ++j) acc[j][f] = mfma16_split<E, !IS_B>(terms, wh[j], wl[j], acc[j][f]);
-      }
-    }
+  // the next block is on its way while the products of this one run
+  WgradBlock<E, RT> even, odd;
+  even.load(side, p.plan.order, first, rank_tiles, j0, c, lane);
+  for (int b = first;;) {
+    odd.load(side, p.plan.order, min(b + 1, last - 1), rank_tiles, j0, c, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    even.template multiply<IS_B>(acc);
+    if (++b >= last) break;
+    even.load(side, p.plan.order, min(b + 1, last - 1), rank_tiles, j0, c, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    odd.template multiply<IS_B>(acc);
+    if (++b >= last) break;
   }
   const int64_t size = static_cast<int64_t>(p.rank) * side.features;
   const int64_t base = (whole ? a : item) * size;
   void *out = whole ? side.grad : side.part;
   const int type = whole ? p.grad_type : kNVTEFloat32;
+  const int r0 = j0 * 16;
 #pragma unroll
   for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -407,12 +535,11 @@ __device__ __forceinline__ void wgrad_side(const WgradArgs &p, const WgradSide &
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
         if constexpr (IS_B) {  // rows are features, columns ranks
-          const int row = c0 + 8 * (4 * (lane >> 4) + i) + f, col = j * 16 + (lane & 15);
-          if (row < side.features && col < ranks) store1(out, base + static_cast<int64_t>(row) * p.rank + j0 + col, type, acc[j][f][i]);
+          const int row = c0 + 8 * (4 * (lane >> 4) + i) + f, col = r0 + j * 16 + (lane & 15);
+          if (row < side.features && col < p.rank) store1(out, base + static_cast<int64_t>(row) * p.rank + col, type, acc[j][f][i]);
         } else {
-          const int row = j * 16 + (lane >> 4) * 4 + i, col = c + f;
-          if (row < ranks && col < side.features)
-            store1(out, base + static_cast<int64_t>(j0 + row) * side.features + col, type, acc[j][f][i]);
+          const int row = r0 + j * 16 + (lane >> 4) * 4 + i, col = c + f;
+          if (row < p.rank && col < side.features) store1(out, base + static_cast<int64_t>(row) * side.features + col, type, acc[j][f][i]);
         }
       }
 }
@@ -420,15 +547,9 @@ __device__ __forceinline__ void wgrad_side(const WgradArgs &p, const WgradSide &
 // grid: column groups of dA, then of dB  x  work items (an upper bound; the rest leave at once)  x  64 ranks
 template <typename E, int RT>
 __global__ __launch_bounds__(256) void wgrad_kernel(WgradArgs p) {
-  __shared__ __attribute__((aligned(16))) uint16_t s_hi[kStep / 32][RT][512], s_lo[kStep / 32][RT][512];
   const int group = blockIdx.x;
-  if (group < p.a.groups) {
-    if (p.a.vec) wgrad_side<E, RT, true, false>(p, p.a, group, s_hi, s_lo);
-    else wgrad_side<E, RT, false, false>(p, p.a, group, s_hi, s_lo);
-  } else {
-    if (p.b.vec) wgrad_side<E, RT, true, true>(p, p.b, group - p.a.groups, s_hi, s_lo);
-    else wgrad_side<E, RT, false, true>(p, p.b, group - p.a.groups, s_hi, s_lo);
-  }
+  if (group < p.a.groups) wgrad_side<E, RT, false>(p, p.a, group);
+  else wgrad_side<E, RT, true>(p, p.b, group - p.a.groups);
 }
 
 // join: the sum of an adapter's work items in their order; zero for an adapter without tokens.  grid: elements x adapters
@@ -441,9 +562,7 @@ __global__ __launch_bounds__(256) void join_kernel(WgradArgs p) {
     const bool is_a = e < size_a;
     const float *part = is_a ? p.a.part : p.b.part;
     const int64_t at = is_a ? e : e - size_a, size = is_a ? size_a : size_b;
-    float s = 0.f;
-    for (int i = 0; i < items; ++i) s += part[(first + i) * size + at];
-    store1(is_a ? p.a.grad : p.b.grad, a * size + at, p.grad_type, s);
+    store1(is_a ? p.a.grad : p.b.grad, a * size + at, p.grad_type, sum_slices(part + first * size + at, items, size));
   }
 }
 
@@ -469,65 +588,83 @@ Shape shape_of(size_t tokens, size_t in, size_t out, size_t rank, size_t num, in
 }
 
 // Few tokens leave most CUs without a tile, so the features are cut into slices (a multiple of 64, at least 256) until about
-// 512 workgroups run; whoever reads the rank vectors adds the slices.
+// 1024 workgroups run; whoever reads the rank vectors adds the slices.
+bool many_tokens(int64_t tokens) { return tokens >= 4096; }
 int slice_of(int64_t tokens, int features) {
-  const int64_t tiles = std::max<int64_t>(1, (tokens + 15) / 16);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(512 / tiles, ceil_div(features, 256)));
+  const int64_t tiles = std::max<int64_t>(1, ceil_div(tokens, many_tokens(tokens) ? 32 : 16));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(1024 / tiles, ceil_div(features, 256)));
   return static_cast<int>(round_up(ceil_div(features, static_cast<size_t>(want)), 64));
 }
 int num_slices(int64_t tokens, int features) { return static_cast<int>(ceil_div(features, slice_of(tokens, features))); }
 
-template <typename E, bool KMAJOR, int RT, int MT, int NW>
-void launch_shrink(const ShrinkArgs &p, int slices, bool vec, hipStream_t stream) {
+template <typename E, int RT, int MT, int NW, int U>
+void launch_shrink(const ShrinkArgs &p, int slices, hipStream_t stream) {
   const int64_t tiles = (p.tokens + 16 * MT - 1) / (16 * MT);
   // a decode tile's adapters go to workgroups of their own while there are too few tiles
   const int64_t most = std::min<int64_t>(std::min<int64_t>(p.num, p.tokens), 16);
   const int64_t phases = std::max<int64_t>(1, std::min<int64_t>(most, 2048 / (tiles * slices)));
-  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, KMAJOR>), dim3(tiles, slices, phases), dim3(NW * 64), 0, stream, p, vec);
+  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, U>), dim3(tiles, slices, phases), dim3(NW * 64), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
-template <typename E, bool KMAJOR>
+template <typename E>
 void shrink(const void *in, const void *pool, const int *ids, float *out, int64_t tokens, int features, int rank, int num,
             hipStream_t stream) {
   const ShrinkArgs p{static_cast<const uint16_t *>(in), static_cast<const uint16_t *>(pool), ids, out, tokens, features, rank, num,
                      slice_of(tokens, features)};
   const int slices = num_slices(tokens, features);
-  const bool vec = features % 8 == 0 && aligned16(in) && (KMAJOR || aligned16(pool));
-  const bool many = tokens >= 4096;
+  const bool many = many_tokens(tokens);
   if (rank <= 16) {
-    many ? launch_shrink<E, KMAJOR, 1, 2, 8>(p, slices, vec, stream) : launch_shrink<E, KMAJOR, 1, 1, 4>(p, slices, vec, stream);
+    many ? launch_shrink<E, 1, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 1, 1, 4, 2>(p, slices, stream);
   } else if (rank <= 32) {
-    many ? launch_shrink<E, KMAJOR, 2, 2, 8>(p, slices, vec, stream) : launch_shrink<E, KMAJOR, 2, 1, 4>(p, slices, vec, stream);
+    many ? launch_shrink<E, 2, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 2, 1, 4, 2>(p, slices, stream);
   } else if (rank <= 64) {
-    launch_shrink<E, KMAJOR, 4, 1, 4>(p, slices, vec, stream);
+    many ? launch_shrink<E, 4, 2, 4, 1>(p, slices, stream) : launch_shrink<E, 4, 1, 4, 1>(p, slices, stream);
   } else {
-    launch_shrink<E, KMAJOR, 8, 1, 4>(p, slices, vec, stream);
+    many ? launch_shrink<E, 8, 2, 4, 1>(p, slices, stream) : launch_shrink<E, 8, 1, 4, 1>(p, slices, stream);
   }
 }
 
-template <typename E, bool RMAJOR, int KT, int MT>
-void launch_expand(ExpandArgs p, bool vec_pool, bool vec_rows, hipStream_t stream) {
-  const int64_t tiles = (p.tokens + 16 * MT - 1) / (16 * MT);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(p.features, 512), 2048 / tiles));
-  p.cols = static_cast<int>(round_up(ceil_div(p.features, static_cast<size_t>(want)), 512));
-  hipLaunchKernelGGL((expand_kernel<E, KT, MT, RMAJOR>), dim3(tiles, ceil_div(p.features, p.cols)), dim3(256), 0, stream, p,
-                     vec_pool, vec_rows);
-  NVTE_CHECK_HIP(hipGetLastError());
+// runs launch(KT, MT) as integral constants: 32 ranks per operand, 16 tokens per tile
+template <typename Launch>
+void expand_variant(int rank, int64_t tokens, Launch &&launch) {
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 2> Two;
+  typedef std::integral_constant<int, 4> Four;
+  const bool many = tokens >= 1024;
+  if (rank <= 32) many ? launch(One(), Two()) : launch(One(), One());
+  else if (rank <= 64) many ? launch(Two(), Two()) : launch(Two(), One());
+  else launch(Four(), One());
 }
 
-template <typename E, bool RMAJOR>
-void expand(const ExpandArgs &p, hipStream_t stream) {
-  const bool vec_pool = (RMAJOR ? p.features : p.rank) % 8 == 0 && aligned16(p.pool);
-  const bool vec_rows = p.features % 8 == 0 && aligned16(p.out) && aligned16(p.base);
-  const bool many = p.tokens >= 1024;
-  if (p.rank <= 32) {
-    many ? launch_expand<E, RMAJOR, 1, 2>(p, vec_pool, vec_rows, stream) : launch_expand<E, RMAJOR, 1, 1>(p, vec_pool, vec_rows, stream);
-  } else if (p.rank <= 64) {
-    many ? launch_expand<E, RMAJOR, 2, 2>(p, vec_pool, vec_rows, stream) : launch_expand<E, RMAJOR, 2, 1>(p, vec_pool, vec_rows, stream);
-  } else {
-    launch_expand<E, RMAJOR, 4, 1>(p, vec_pool, vec_rows, stream);
-  }
+// columns per workgroup: 512 until there are about 2048 workgroups
+int columns_of(int64_t tiles, int features) {
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(features, 512), 2048 / tiles));
+  return static_cast<int>(round_up(ceil_div(features, static_cast<size_t>(want)), 512));
+}
+
+template <typename E>
+void expand(ExpandArgs p, hipStream_t stream) {
+  expand_variant(p.rank, p.tokens, [&](auto kt, auto mt) {
+    const int64_t tiles = ceil_div(p.tokens, 16 * mt());
+    p.cols = columns_of(tiles, p.features);
+    hipLaunchKernelGGL((expand_kernel<E, kt(), mt(), false>), dim3(tiles, ceil_div(p.features, p.cols)), dim3(256), 0, stream, p);
+    NVTE_CHECK_HIP(hipGetLastError());
+  });
+}
+
+template <typename E>
+void expand_and_pack(ExpandArgs p, const PackArgs &q, int64_t blocks, hipStream_t stream) {
+  expand_variant(p.rank, p.tokens, [&](auto kt, auto mt) {
+    const int64_t tiles = ceil_div(p.tokens, 16 * mt());
+    p.cols = columns_of(tiles, p.features);
+    const int64_t ranges = p.out != nullptr ? ceil_div(p.features, p.cols) : 0, grid = 2 * blocks + tiles * ranges;
+    NVTE_CHECK(grid <= INT_MAX, "too many workgroups: ", grid);
+    if (grid == 0) return;
+    hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt()>), dim3(grid), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
+                       static_cast<int>(tiles), static_cast<int>(blocks));
+    NVTE_CHECK_HIP(hipGetLastError());
+  });
 }
 
 template <typename E>
@@ -539,16 +676,18 @@ void launch_wgrad(const WgradArgs &p, unsigned items, hipStream_t stream) {
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
-// how many tokens a work item sums: enough items for about four waves per CU, no fewer than 64 tokens each
-int tokens_per_item(const Shape &s) {
+// how many blocks of 32 tokens a work item sums: enough items for about eight waves per CU
+int blocks_per_item(const Shape &s) {
   const int64_t columns = ceil_div(s.in, 512) + ceil_div(s.out, 512);
   const int64_t items = std::max<int64_t>(1, 512 / columns);
-  return static_cast<int>(round_up(std::max<size_t>(64, ceil_div(s.tokens, items)), 64));
+  return static_cast<int>(std::max<size_t>(2, ceil_div(ceil_div(s.tokens, kBlock), items)));
 }
-int64_t most_items(const Shape &s) { return s.tokens / tokens_per_item(s) + std::min<int64_t>(s.num, s.tokens); }
+// every adapter's last block (item) may be partly filled
+int64_t most_blocks(const Shape &s) { return s.tokens / kBlock + std::min<int64_t>(s.num, s.tokens); }
+int64_t most_items(const Shape &s) { return most_blocks(s) / blocks_per_item(s) + std::min<int64_t>(s.num, s.tokens); }
 
 struct BackwardWorkspace {
-  size_t low, order, token_base, item_base, part_a, part_b, bytes;
+  size_t low, transposed, order, block_base, item_base, packed_a, packed_b, part_a, part_b, bytes;
 };
 BackwardWorkspace backward_workspace(const Shape &s) {
   BackwardWorkspace w{};
@@ -559,9 +698,13 @@ BackwardWorkspace backward_workspace(const Shape &s) {
     return here;
   };
   w.low = take(static_cast<size_t>(num_slices(s.tokens, s.out)) * s.tokens * s.rank * sizeof(float));
-  w.order = take(s.tokens * sizeof(int));
-  w.token_base = take((s.num + 1) * sizeof(int));
+  w.transposed = take(static_cast<size_t>(s.num) * s.rank * s.out * 2);
+  w.order = take(most_blocks(s) * kBlock * sizeof(int));
+  w.block_base = take((s.num + 1) * sizeof(int));
   w.item_base = take((s.num + 1) * sizeof(int));
+  const size_t packed = static_cast<size_t>(most_blocks(s)) * ceil_div(s.rank, 16) * 2048;
+  w.packed_a = take(packed);
+  w.packed_b = take(packed);
   w.part_a = take(static_cast<size_t>(most_items(s)) * s.rank * s.in * sizeof(float));
   w.part_b = take(static_cast<size_t>(most_items(s)) * s.rank * s.out * sizeof(float));
   w.bytes = at;
@@ -573,33 +716,44 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
               const float *low, const void *base_grad, void *dx, void *da, void *db, int grad_type, char *ws, hipStream_t stream) {
   const BackwardWorkspace w = backward_workspace(s);
   float *up = reinterpret_cast<float *>(ws + w.low);
+  uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
+  const Plan plan{reinterpret_cast<int *>(ws + w.order), reinterpret_cast<int *>(ws + w.block_base),
+                  reinterpret_cast<int *>(ws + w.item_base)};
+  const bool wgrad = da != nullptr;
+  if (!wgrad && (dx == nullptr || s.tokens == 0)) return;
+  const int per_item = blocks_per_item(s);
+  const int64_t pieces = s.tokens > 0 ? static_cast<int64_t>(s.num) * ceil_div(s.out, 64) : 0, lists = wgrad ? s.num : 0;
+  NVTE_CHECK(lists + pieces <= INT_MAX, "too many adapters: ", s.num);
+  const PrepareArgs prep{ids, static_cast<const uint16_t *>(b), bt, plan, s.tokens, s.out, s.rank, s.num, per_item, static_cast<int>(lists)};
+  hipLaunchKernelGGL(prepare_kernel, dim3(lists + pieces), dim3(1024), 0, stream, prep);
+  NVTE_CHECK_HIP(hipGetLastError());
+  const int64_t blocks = wgrad ? most_blocks(s) : 0;
+  uint16_t *packed_a = reinterpret_cast<uint16_t *>(ws + w.packed_a), *packed_b = reinterpret_cast<uint16_t *>(ws + w.packed_b);
   if (s.tokens > 0) {
-    shrink<E, true>(dy, b, ids, up, s.tokens, s.out, s.rank, s.num, stream);
-    if (dx != nullptr)
-      expand<E, true>({up, static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(base_grad), scaling, ids,
-                       static_cast<uint16_t *>(dx), s.tokens, num_slices(s.tokens, s.out), s.in, s.rank, s.num, 0}, stream);
+    shrink<E>(dy, bt, ids, up, s.tokens, s.out, s.rank, s.num, stream);
+    const ExpandArgs e{up, static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(base_grad), scaling, ids,
+                       static_cast<uint16_t *>(dx), s.tokens, num_slices(s.tokens, s.out), s.in, s.rank, s.num, 0};
+    const PackArgs q{{{up, packed_a, num_slices(s.tokens, s.out)}, {low, packed_b, num_slices(s.tokens, s.in)}}, scaling, plan,
+                     s.tokens, s.rank, s.num};
+    expand_and_pack<E>(e, q, blocks, stream);
   }
-  if (da == nullptr) return;
+  if (!wgrad) return;
   WgradArgs p{};
-  p.a = {static_cast<const uint16_t *>(x), up, da, reinterpret_cast<float *>(ws + w.part_a), num_slices(s.tokens, s.out), s.in,
-         static_cast<int>(ceil_div(s.in, 512)), s.in % 8 == 0 && aligned16(x)};
-  p.b = {static_cast<const uint16_t *>(dy), low, db, reinterpret_cast<float *>(ws + w.part_b), num_slices(s.tokens, s.in), s.out,
-         static_cast<int>(ceil_div(s.out, 512)), s.out % 8 == 0 && aligned16(dy)};
-  p.scaling = scaling;
-  p.plan = {reinterpret_cast<int *>(ws + w.order), reinterpret_cast<int *>(ws + w.token_base), reinterpret_cast<int *>(ws + w.item_base)};
-  p.tokens = s.tokens;
+  p.a = {static_cast<const uint16_t *>(x), packed_a, da, reinterpret_cast<float *>(ws + w.part_a), s.in,
+         static_cast<int>(ceil_div(s.in, 512))};
+  p.b = {static_cast<const uint16_t *>(dy), packed_b, db, reinterpret_cast<float *>(ws + w.part_b), s.out,
+         static_cast<int>(ceil_div(s.out, 512))};
+  p.plan = plan;
   p.rank = s.rank;
   p.num = s.num;
-  p.per_item = tokens_per_item(s);
+  p.per_item = per_item;
   p.grad_type = grad_type;
-  hipLaunchKernelGGL(plan_kernel, dim3(s.num), dim3(256), 0, stream, ids, s.tokens, s.num, p.per_item, p.plan);
-  NVTE_CHECK_HIP(hipGetLastError());
   const int64_t items = most_items(s);
   NVTE_CHECK(items <= 65535, "too many work items: ", items);
   if (items > 0) launch_wgrad<E>(p, static_cast<unsigned>(items), stream);
   const int64_t elements = static_cast<int64_t>(s.rank) * (static_cast<int64_t>(s.in) + s.out);
-  const int64_t blocks = std::min<int64_t>(ceil_div(elements, 256), std::max<int64_t>(1, 4096 / s.num));
-  hipLaunchKernelGGL(join_kernel, dim3(blocks, s.num), dim3(256), 0, stream, p);
+  const int64_t grid = std::min<int64_t>(ceil_div(elements, 256), std::max<int64_t>(1, 4096 / s.num));
+  hipLaunchKernelGGL(join_kernel, dim3(grid, s.num), dim3(256), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
@@ -627,11 +781,11 @@ void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const in
     const ExpandArgs p{low, static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(base), scaling, adapter_ids,
                        static_cast<uint16_t *>(out), s.tokens, num_slices(s.tokens, s.in), s.out, s.rank, s.num, 0};
     if (s.type == kNVTEBFloat16) {
-      shrink<bf16_t, false>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
-      expand<bf16_t, false>(p, stream);
+      shrink<bf16_t>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
+      expand<bf16_t>(p, stream);
     } else {
-      shrink<f16_t, false>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
-      expand<f16_t, false>(p, stream);
+      shrink<f16_t>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
+      expand<f16_t>(p, stream);
     }
   });
 }

@@ -18,6 +18,12 @@ namespace te {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// The matrix instructions ignore the lane mask, so what loops and branches around them depend on is made scalar, the wave's own
+// number first.  And no branch skips one matrix instruction between others: where the skipped part writes other registers, this
+// compiler (ROCm 7.2) counts the wait states of the joining block's reads along the long path only, and the short path reads a
+// result before it is there.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 template <typename E>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
 template <>
@@ -78,17 +84,26 @@ __device__ __forceinline__ f32x4 mfma16_split(const Terms<E> &w, u32x4 hi, u32x4
   }
 }
 
-// elements k .. k + 7 of a row of `n` 16-bit elements, zero from n on; VEC: n % 8 == 0 and the row is 16-byte aligned
-template <bool VEC>
-__device__ __forceinline__ u32x4 row8(const uint16_t *row, int64_t k, int64_t n) {
+// Eight 16-bit elements at any element address: the hardware takes unaligned 16-byte global accesses, so neither odd row
+// lengths nor shifted storage need kernels of their own.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ u32x4 load8(const uint16_t *p) { return *reinterpret_cast<const u32x4_any *>(p); }
+__device__ __forceinline__ void store8(uint16_t *p, u32x4 v) { *reinterpret_cast<u32x4_any *>(p) = v; }
+// the first `valid` of them, zeros after; nothing behind p + valid is touched
+__device__ __forceinline__ u32x4 load8_head(const uint16_t *p, int valid) {
+  if (valid >= 8) return load8(p);
   u32x4 v = {0u, 0u, 0u, 0u};
-  if constexpr (VEC) {
-    if (k < n) v = *reinterpret_cast<const u32x4 *>(row + k);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < n) v[i >> 1] |= static_cast<uint32_t>(row[k + i]) << (16 * (i & 1));
-  }
+  for (int i = 0; i < 7; ++i)
+    if (i < valid) v[i >> 1] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
+  return v;
+}
+// the same where p + 8 may reach into memory of the same array that ends at `end`: one access and a mask away from its end
+__device__ __forceinline__ u32x4 load8_head(const uint16_t *p, int valid, const uint16_t *end) {
+  if (valid >= 8 || p + 8 > end) return load8_head(p, valid);
+  u32x4 v = load8(p);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) v[w] &= valid > 2 * w + 1 ? 0xFFFFFFFFu : valid > 2 * w ? 0xFFFFu : 0u;
   return v;
 }
 

@@ -3,6 +3,7 @@
 //   p = softmax(logits[t]);  ids = the top_k largest (ties: lowest index);  weights = p[ids], or p[ids] / sum p[ids]
 //   h[t, j] = silu(W1[e, :F] x[t]) * (W1[e, F:] x[t]),   out[t] = sum_j weights[t, j] W2[e] h[t, j],   e = ids[t, j]
 //
+// Token slots of a tile that no token fills read the expert's last one again and their results are dropped.
 // A decode batch is bound by the weights of the experts it hits (3 F H values each, read once): a workgroup owns 16 rows of one
 // expert's matrix, finds that expert's tokens itself by scanning the routing table (T * top_k <= 4096 entries, out of cache) and
 // leaves at once if there are none, so the host never learns the routing and nothing has to be sorted first.  The weights are
@@ -33,6 +34,42 @@ struct fp8_t {
 };
 
 // ------------------------------------------------------------------------------------------------ router
+// value order in the high word (NaN below everything), lower index first in the low word; never 0
+__device__ __forceinline__ uint64_t order_key(float v, int e) {
+  const uint32_t b = __float_as_uint(v);
+  const uint32_t order = v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~e);
+}
+
+// up to 64 experts, one wave per token, one logit per lane: a lane's rank is the number of larger keys
+__global__ __launch_bounds__(256) void topk64_kernel(const void *logits, int dtype, int *ids, float *weights, int64_t tokens,
+                                                     int experts, int top_k, bool renormalize) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (t >= tokens) return;
+  const bool mine = lane < experts;
+  const float v = mine ? load1(logits, t * experts + lane, dtype) + 0.f : -__builtin_inff();  // -0 becomes +0: they tie
+  const uint64_t key = mine ? order_key(v, lane) : 0;
+  const uint32_t hi = static_cast<uint32_t>(key >> 32), lo = static_cast<uint32_t>(key);
+  int rank = 0;
+#pragma unroll 8
+  for (int e = 0; e < experts; ++e) {
+    const uint64_t other = (static_cast<uint64_t>(__builtin_amdgcn_readlane(hi, e)) << 32) |
+                           static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, e));
+    rank += other > key;
+  }
+  const bool chosen = mine && rank < top_k;
+  const float top = wave_max(v);
+  const float x = mine ? expf(v - top) : 0.f;
+  float total = renormalize && !chosen ? 0.f : x;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+  if (chosen) {
+    ids[t * top_k + rank] = lane;
+    weights[t * top_k + rank] = x / total;
+  }
+}
+
 // one wave per token, N logits per lane
 template <int N>
 __global__ __launch_bounds__(256) void topk_kernel(const void *logits, int dtype, int *ids, float *weights, int64_t tokens,
@@ -41,7 +78,7 @@ __global__ __launch_bounds__(256) void topk_kernel(const void *logits, int dtype
   const int64_t t = blockIdx.x * 4ll + (threadIdx.x >> 6);
   if (t >= tokens) return;
   float v[N];
-  uint64_t key[N];  // value order in the high word (NaN below everything), lower index first in the low word; 0 = none
+  uint64_t key[N];  // 0 = none
   float top = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -50,9 +87,7 @@ __global__ __launch_bounds__(256) void topk_kernel(const void *logits, int dtype
     v[i] = -__builtin_inff();
     if (e < experts) {
       v[i] = load1(logits, t * experts + e, dtype) + 0.f;  // -0 becomes +0: they tie
-      const uint32_t b = __float_as_uint(v[i]);
-      const uint32_t order = v[i] != v[i] ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-      key[i] = (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~e);
+      key[i] = order_key(v[i], e);
       top = fmaxf(top, v[i]);
     }
   }
@@ -91,9 +126,10 @@ __global__ __launch_bounds__(256) void topk_kernel(const void *logits, int dtype
 }
 
 // ------------------------------------------------------------------------------------------------ expert products
-// sixteen weights of one row at k .. k + 15, as two operands of eight in E's format
+// Thirty-two bytes of a weight row per lane: the four lane groups of a wave cover one 128-byte line of each of 16 rows.
+// `operands` widens them to matrix operands of eight k each (in E's format, exact).
 template <typename E>
-__device__ __forceinline__ u32x2 widen4(uint32_t w);  // four FP8 (E4M3) -> four E, exact
+__device__ __forceinline__ u32x2 widen4(uint32_t w);  // four FP8 (E4M3) -> four E
 template <>
 __device__ __forceinline__ u32x2 widen4<bf16_t>(uint32_t w) {
   return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false)),
@@ -106,42 +142,50 @@ __device__ __forceinline__ u32x2 widen4<f16_t>(uint32_t w) {
 }
 
 template <typename W>
-struct Raw16;
+struct Line;
 template <>
-struct Raw16<uint16_t> {
+struct Line<uint16_t> {
+  static constexpr int kOps = 2;      // operands per lane
+  static constexpr int kBlock = 64;   // k per wave
   u32x4 v[2];
-  template <bool VEC>
-  static __device__ __forceinline__ Raw16 load(const uint16_t *row, int64_t k, int64_t n) {
-    return {{row8<VEC>(row, k, n), row8<VEC>(row, k + 8, n)}};
+  __device__ __forceinline__ void load(const uint16_t *p) {
+    v[0] = load8(p);
+    v[1] = load8(p + 8);
+  }
+  __device__ __forceinline__ void load_head(const uint16_t *p, int valid) {
+    v[0] = load8_head(p, valid);
+    v[1] = load8_head(p + 8, valid - 8);
   }
   template <typename E>
-  __device__ __forceinline__ void operands(u32x4 (&o)[2]) const {
-    o[0] = v[0];
-    o[1] = v[1];
+  __device__ __forceinline__ u32x4 operand(int i) const {
+    return v[i];
   }
 };
 template <>
-struct Raw16<fp8_t> {
-  u32x4 v;
-  template <bool VEC>
-  static __device__ __forceinline__ Raw16 load(const fp8_t *row, int64_t k, int64_t n) {
-    Raw16 r{{0u, 0u, 0u, 0u}};
-    if constexpr (VEC) {
-      if (k < n) r.v = *reinterpret_cast<const u32x4 *>(row + k);
-    } else {
+struct Line<fp8_t> {
+  static constexpr int kOps = 4;
+  static constexpr int kBlock = 128;
+  typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
+  u32x4 v[2];
+  __device__ __forceinline__ void load(const fp8_t *p) {
+    v[0] = *reinterpret_cast<const any *>(p);
+    v[1] = *reinterpret_cast<const any *>(p + 16);
+  }
+  __device__ __forceinline__ void load_head(const fp8_t *p, int valid) {
+    if (valid >= 32) return load(p);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (k + i < n) r.v[i >> 2] |= static_cast<uint32_t>(row[k + i].bits) << (8 * (i & 3));
+    for (int w = 0; w < 8; ++w) {
+      uint32_t d = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * w + i < valid) d |= static_cast<uint32_t>(p[4 * w + i].bits) << (8 * i);
+      v[w >> 2][w & 3] = d;
     }
-    return r;
   }
   template <typename E>
-  __device__ __forceinline__ void operands(u32x4 (&o)[2]) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x2 a = widen4<E>(v[2 * h]), b = widen4<E>(v[2 * h + 1]);
-      o[h] = u32x4{a[0], a[1], b[0], b[1]};
-    }
+  __device__ __forceinline__ u32x4 operand(int i) const {
+    const u32x2 a = widen4<E>(v[i >> 1][2 * (i & 1)]), b = widen4<E>(v[i >> 1][2 * (i & 1) + 1]);
+    return u32x4{a[0], a[1], b[0], b[1]};
   }
 };
 
@@ -164,6 +208,32 @@ __device__ __forceinline__ int find_pairs(const int *ids, int pairs, int e, uint
   return n;
 }
 
+// The blocks of k of one of KW waves (every KW-th), U at a time, every load of them on its way before the first product waits.  What is
+// left over goes singly, the row's ragged end last.  Stage<U, GUARD>: load(block) and multiply(acc).
+template <int U, int KW, template <int, bool> class Stage, typename Args, typename Acc>
+__device__ __forceinline__ void for_blocks(const Args &args, int k, int block, int first, Acc &acc) {
+  const int full = k / block;
+  int b = first;
+  for (; b + KW * (U - 1) < full; b += KW * U) {
+    Stage<U, false> s;
+    s.load(args, b);
+    __builtin_amdgcn_sched_barrier(0);
+    s.multiply(args, acc);
+  }
+  if constexpr (U > 1) {
+    for (; b < full; b += KW) {
+      Stage<1, false> s;
+      s.load(args, b);
+      s.multiply(args, acc);
+    }
+  }
+  if (b == full && k % block != 0) {
+    Stage<1, true> s;
+    s.load(args, b);
+    s.multiply(args, acc);
+  }
+}
+
 struct Fc1Args {
   const void *x, *w;       // [tokens][hidden], [experts][2 ffn][hidden]
   const float *scale_inv;  // [experts], null: 1
@@ -172,86 +242,135 @@ struct Fc1Args {
   int pairs, top_k, hidden, ffn;
 };
 
-template <typename W, typename E, int MT, bool VEC>
-__device__ __forceinline__ void fc1_sum(const Fc1Args &p, const W *gate, const W *up, const uint16_t *const (&row)[MT], int tiles,
-                                        int wave, int lane, f32x4 (&acc)[2][MT]) {
-  for (int k0 = wave * 64; k0 < p.hidden; k0 += kWaves * 64) {
-    const int k = k0 + 16 * (lane >> 4);
-    const Raw16<W> g = Raw16<W>::template load<VEC>(gate, k, p.hidden), u = Raw16<W>::template load<VEC>(up, k, p.hidden);
-    u32x4 x[MT][2];
+template <typename W, typename E, int MT, int FT, int KW>
+struct Fc1 {
+  const W *gate[FT];        // this lane's rows of the gate half
+  int64_t up;               // from there to the other half's
+  const uint16_t *row[MT];  // this lane's tokens
+  int hidden, lane;
+
+  template <int U, bool GUARD>
+  struct Stage {
+    typedef Line<W> L;
+    static constexpr int N = L::kOps;
+    L g[U][FT], u[U][FT];
+    u32x4 x[U][MT][N];
+    __device__ __forceinline__ void load(const Fc1 &p, int block) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < tiles) {
-        x[m][0] = row8<VEC>(row[m], k, p.hidden);
-        x[m][1] = row8<VEC>(row[m], k + 8, p.hidden);
-      }
-    u32x4 go[2], uo[2];
-    g.template operands<E>(go);
-    u.template operands<E>(uo);
+      for (int s = 0; s < U; ++s) {
+        const int k = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < tiles) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          acc[0][m] = mfma16<E>(go[h], x[m][h], acc[0][m]);
-          acc[1][m] = mfma16<E>(uo[h], x[m][h], acc[1][m]);
+        for (int f = 0; f < FT; ++f) {
+          if constexpr (GUARD) {
+            g[s][f].load_head(p.gate[f] + k, p.hidden - k);
+            u[s][f].load_head(p.gate[f] + p.up + k, p.hidden - k);
+          } else {
+            g[s][f].load(p.gate[f] + k);
+            u[s][f].load(p.gate[f] + p.up + k);
+          }
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int o = 0; o < N; ++o) {
+            if constexpr (GUARD) x[s][m][o] = load8_head(p.row[m] + k + 8 * o, p.hidden - k - 8 * o);
+            else x[s][m][o] = load8(p.row[m] + k + 8 * o);
+          }
+      }
+    }
+    __device__ __forceinline__ void multiply(const Fc1 &p, f32x4 (&acc)[FT * MT * 2]) const {
+#pragma unroll
+      for (int s = 0; s < U; ++s)
+#pragma unroll
+        for (int o = 0; o < N; ++o)
+#pragma unroll
+          for (int f = 0; f < FT; ++f) {
+            const u32x4 go = g[s][f].template operand<E>(o), uo = u[s][f].template operand<E>(o);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              f32x4 *a = acc + 2 * (f * MT + m);
+              a[0] = mfma16<E>(go, x[s][m][o], a[0]);
+              a[1] = mfma16<E>(uo, x[s][m][o], a[1]);
+            }
+          }
+    }
+  };
+};
+
+// Sum over the KW waves that share a row group's k; D's registers as they are: token = lane % 16, rows 4 (lane / 16) + i.
+template <int KW, int N>
+__device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*red)[64], int wave, int lane) {
+  if constexpr (KW > 1) {
+    __syncthreads();  // the last join's sums are read
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[wave * N + i][lane] = acc[i];
+    __syncthreads();
+    // each wave adds up its share of the group's registers
+    const int first = wave / KW * KW;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i % KW == wave % KW) {
+        f32x4 s = red[first * N + i][lane];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) s += red[(first + w) * N + i][lane];
+        acc[i] = s;
       }
   }
 }
 
-// grid: 16 rows of the gate half (and the same of the other) x experts
-template <typename W, typename E, int MT>
-__global__ __launch_bounds__(256) void fc1_kernel(Fc1Args p, bool vec) {
+// grid: (4 / KW) 16 FT rows of the gate half (and the same of the other) x experts
+template <typename W, typename E, int MT, int FT, int U, int KW>
+__global__ __launch_bounds__(256) void fc1_kernel(Fc1Args p) {
   __shared__ uint16_t list[kMaxPairs];
   __shared__ int scratch[kWaves];
-  __shared__ float red[kWaves][2 * MT * 256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int e = blockIdx.y, f0 = blockIdx.x * 16;
-  const int n = find_pairs(p.ids, p.pairs, e, list, scratch);
-  const int f_row = min(f0 + (lane & 15), p.ffn - 1);
+  __shared__ f32x4 red[KW > 1 ? kWaves * 2 * FT * MT : 1][64];
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const int e = blockIdx.y, f0 = (blockIdx.x * (kWaves / KW) + wave / KW) * (16 * FT);
+  const int n = __builtin_amdgcn_readfirstlane(find_pairs(p.ids, p.pairs, e, list, scratch));
+  if (n == 0) return;
   const W *w = static_cast<const W *>(p.w) + static_cast<int64_t>(e) * 2 * p.ffn * p.hidden;
-  const W *gate = w + static_cast<int64_t>(f_row) * p.hidden, *up = gate + static_cast<int64_t>(p.ffn) * p.hidden;
+  typedef Fc1<W, E, MT, FT, KW> Side;
+  Side side;
+  side.up = static_cast<int64_t>(p.ffn) * p.hidden;
+  side.hidden = p.hidden;
+  side.lane = lane;
+#pragma unroll
+  for (int f = 0; f < FT; ++f) side.gate[f] = w + static_cast<int64_t>(min(f0 + f * 16 + (lane & 15), p.ffn - 1)) * p.hidden;
   const float scale = p.scale_inv != nullptr ? p.scale_inv[e] : 1.f;
   for (int n0 = 0; n0 < n; n0 += 16 * MT) {
-    const uint16_t *row[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int pair = list[min(n0 + m * 16 + (lane & 15), n - 1)];
-      row[m] = static_cast<const uint16_t *>(p.x) + static_cast<int64_t>(pair / p.top_k) * p.hidden;
+      side.row[m] = static_cast<const uint16_t *>(p.x) + static_cast<int64_t>(pair / p.top_k) * p.hidden;
     }
-    const int tiles = min(MT, (n - n0 + 15) / 16);
-    f32x4 acc[2][MT] = {};
-    if (vec) fc1_sum<W, E, MT, true>(p, gate, up, row, tiles, wave, lane, acc);
-    else fc1_sum<W, E, MT, false>(p, gate, up, row, tiles, wave, lane, acc);
+    f32x4 acc[FT * MT * 2] = {};  // [f][m][gate, up]
+    for_blocks<U, KW, Side::template Stage>(side, p.hidden, Line<W>::kBlock, wave % KW, acc);
+    // gate and up of one tile stay with one wave
+    f32x4 g[FT * MT], u[FT * MT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < FT * MT; ++i) {
+      g[i] = acc[2 * i];
+      u[i] = acc[2 * i + 1];
+    }
+    join_waves<KW>(g, red, wave, lane);
+    join_waves<KW>(u, red, wave, lane);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < FT * MT; ++i) {
+      const int f = i / MT, m = i % MT;
+      const int at = n0 + m * 16 + (lane & 15), col = f0 + f * 16 + (lane >> 4) * 4;
+      if (i % KW != wave % KW || at >= n) continue;
+      const int64_t o = static_cast<int64_t>(list[at]) * p.ffn + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][((s * MT + m) * 4 + i) * 64 + lane] = acc[s][m][i];
-    __syncthreads();
-    for (int q = threadIdx.x; q < tiles * 256; q += 256) {
-      const int f = q & 15, tok = (q >> 4) & 15, m = q >> 8;
-      const int slot = (m * 4 + (f & 3)) * 64 + (f >> 2) * 16 + tok;
-      float g = 0.f, u = 0.f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
-        g += red[v][slot];
-        u += red[v][MT * 256 + slot];
-      }
-      g *= scale;
-      u *= scale;
-      const int at = n0 + m * 16 + tok;
-      if (at < n && f0 + f < p.ffn) {
+      for (int r = 0; r < 4; ++r) {
+        const float a = g[i][r] * scale, b = u[i][r] * scale;
         __bf16 hi, lo;
-        split1(g * sigmoid_f(g) * u, hi, lo);
-        const int64_t o = static_cast<int64_t>(list[at]) * p.ffn + f0 + f;
-        p.h_hi[o] = bits16(hi);
-        p.h_lo[o] = bits16(lo);
+        split1(a * sigmoid_f(a) * b, hi, lo);
+        if (col + r < p.ffn) {
+          p.h_hi[o + r] = bits16(hi);
+          p.h_lo[o + r] = bits16(lo);
+        }
       }
     }
-    __syncthreads();
   }
 }
 
@@ -265,80 +384,103 @@ struct Fc2Args {
   int pairs, hidden, ffn;
 };
 
-// eight stored weights as bf16 terms: FP8 is widened first (exact), 16-bit types as they are
+// the format in which stored weights meet h's bf16 terms: FP8 is widened (exact), 16-bit types stay
 template <typename W, typename E>
-struct Fc2Terms {
+struct Fc2Type {
   typedef E type;
 };
 template <typename E>
-struct Fc2Terms<fp8_t, E> {
+struct Fc2Type<fp8_t, E> {
   typedef bf16_t type;
 };
 
-template <typename W, typename E, int MT, bool VEC>
-__device__ __forceinline__ void fc2_sum(const Fc2Args &p, const W *w, const int64_t (&row)[MT], int tiles, int wave, int lane,
-                                        f32x4 (&acc)[MT]) {
-  typedef typename Fc2Terms<W, E>::type T;
-  for (int k0 = wave * 64; k0 < p.ffn; k0 += kWaves * 64) {
-    const int k = k0 + 16 * (lane >> 4);
-    const Raw16<W> r = Raw16<W>::template load<VEC>(w, k, p.ffn);
-    u32x4 hi[MT][2], lo[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (m < tiles) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          hi[m][h] = row8<VEC>(p.h_hi + row[m], k + 8 * h, p.ffn);
-          lo[m][h] = row8<VEC>(p.h_lo + row[m], k + 8 * h, p.ffn);
-        }
-      }
-    u32x4 o[2];
-    r.template operands<T>(o);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Terms<T> terms(o[h]);
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (m < tiles) acc[m] = mfma16_split<T>(terms, hi[m][h], lo[m][h], acc[m]);
-    }
-  }
-}
+template <typename W, typename E, int MT, int FT, int KW>
+struct Fc2 {
+  const W *w[FT];                // this lane's rows
+  const uint16_t *hi[MT];        // this lane's tokens
+  int64_t lo;                    // from hi to their second terms
+  int ffn, lane;
 
-// grid: 16 rows of the output x experts
-template <typename W, typename E, int MT>
-__global__ __launch_bounds__(256) void fc2_kernel(Fc2Args p, bool vec) {
+  template <int U, bool GUARD>
+  struct Stage {
+    typedef Line<W> L;
+    typedef typename Fc2Type<W, E>::type T;
+    static constexpr int N = L::kOps;
+    L r[U][FT];
+    u32x4 h[U][MT][N][2];
+    __device__ __forceinline__ void load(const Fc2 &p, int block) {
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        const int k = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+          if constexpr (GUARD) r[s][f].load_head(p.w[f] + k, p.ffn - k);
+          else r[s][f].load(p.w[f] + k);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int o = 0; o < N; ++o)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint16_t *at = p.hi[m] + t * p.lo + k + 8 * o;
+              if constexpr (GUARD) h[s][m][o][t] = load8_head(at, p.ffn - k - 8 * o);
+              else h[s][m][o][t] = load8(at);
+            }
+      }
+    }
+    __device__ __forceinline__ void multiply(const Fc2 &p, f32x4 (&acc)[FT * MT]) const {
+#pragma unroll
+      for (int s = 0; s < U; ++s)
+#pragma unroll
+        for (int o = 0; o < N; ++o)
+#pragma unroll
+          for (int f = 0; f < FT; ++f) {
+            const Terms<T> terms(r[s][f].template operand<T>(o));
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[f * MT + m] = mfma16_split<T>(terms, h[s][m][o][0], h[s][m][o][1], acc[f * MT + m]);
+          }
+    }
+  };
+};
+
+// grid: (4 / KW) 16 FT rows of the output x experts
+template <typename W, typename E, int MT, int FT, int U, int KW>
+__global__ __launch_bounds__(256) void fc2_kernel(Fc2Args p) {
   __shared__ uint16_t list[kMaxPairs];
   __shared__ int scratch[kWaves];
-  __shared__ float red[kWaves][MT * 256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int e = blockIdx.y, c0 = blockIdx.x * 16;
-  const int n = find_pairs(p.ids, p.pairs, e, list, scratch);
-  const int c_row = min(c0 + (lane & 15), p.hidden - 1);
-  const W *w = static_cast<const W *>(p.w) + (static_cast<int64_t>(e) * p.hidden + c_row) * p.ffn;
+  __shared__ f32x4 red[KW > 1 ? kWaves * FT * MT : 1][64];
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const int e = blockIdx.y, c0 = (blockIdx.x * (kWaves / KW) + wave / KW) * (16 * FT);
+  const int n = __builtin_amdgcn_readfirstlane(find_pairs(p.ids, p.pairs, e, list, scratch));
+  if (n == 0) return;
+  typedef Fc2<W, E, MT, FT, KW> Side;
+  Side side;
+  side.lo = p.h_lo - p.h_hi;
+  side.ffn = p.ffn;
+  side.lane = lane;
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+    side.w[f] = static_cast<const W *>(p.w) + (static_cast<int64_t>(e) * p.hidden + min(c0 + f * 16 + (lane & 15), p.hidden - 1)) * p.ffn;
   const float scale = p.scale_inv != nullptr ? p.scale_inv[e] : 1.f;
   for (int n0 = 0; n0 < n; n0 += 16 * MT) {
-    int64_t row[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) row[m] = static_cast<int64_t>(list[min(n0 + m * 16 + (lane & 15), n - 1)]) * p.ffn;
-    const int tiles = min(MT, (n - n0 + 15) / 16);
-    f32x4 acc[MT] = {};
-    if (vec) fc2_sum<W, E, MT, true>(p, w, row, tiles, wave, lane, acc);
-    else fc2_sum<W, E, MT, false>(p, w, row, tiles, wave, lane, acc);
+    for (int m = 0; m < MT; ++m) side.hi[m] = p.h_hi + static_cast<int64_t>(list[min(n0 + m * 16 + (lane & 15), n - 1)]) * p.ffn;
+    f32x4 acc[FT * MT] = {};
+    for_blocks<U, KW, Side::template Stage>(side, p.ffn, Line<W>::kBlock, wave % KW, acc);
+    join_waves<KW>(acc, red, wave, lane);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < FT * MT; ++i) {
+      const int f = i / MT, m = i % MT;
+      const int at = n0 + m * 16 + (lane & 15), col = c0 + f * 16 + (lane >> 4) * 4;
+      if (i % KW != wave % KW || at >= n) continue;
+      const float factor = scale * p.weights[list[at]];
+      float *y = p.y + static_cast<int64_t>(list[at]) * p.hidden + col;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[wave][(m * 4 + i) * 64 + lane] = acc[m][i];
-    __syncthreads();
-    for (int q = threadIdx.x; q < tiles * 256; q += 256) {
-      const int c = q & 15, tok = (q >> 4) & 15, m = q >> 8;
-      const int slot = (m * 4 + (c & 3)) * 64 + (c >> 2) * 16 + tok;
-      float y = 0.f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) y += red[v][slot];
-      const int at = n0 + m * 16 + tok;
-      if (at < n && c0 + c < p.hidden) p.y[static_cast<int64_t>(list[at]) * p.hidden + c0 + c] = y * scale * p.weights[list[at]];
+      for (int r = 0; r < 4; ++r)
+        if (col + r < p.hidden) y[r] = acc[i][r] * factor;
     }
-    __syncthreads();
   }
 }
 
@@ -349,9 +491,16 @@ __global__ __launch_bounds__(256) void combine_kernel(const float *y, const int 
   const int64_t t = blockIdx.y;
   if (c >= hidden) return;
   float s = 0.f;
-  for (int j = 0; j < top_k; ++j) {
-    const int id = ids[t * top_k + j];
-    if (id >= 0 && id < experts) s += y[(t * top_k + j) * hidden + c];
+  for (int j0 = 0; j0 < top_k; j0 += 8) {  // eight at a time on their way
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = min(j0 + i, top_k - 1), id = ids[t * top_k + j];
+      const bool there = j0 + i < top_k && id >= 0 && id < experts;
+      v[i] = there ? y[(t * top_k + j) * hidden + c] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
   }
   narrow(s, out[t * hidden + c]);
 }
@@ -378,14 +527,11 @@ Layer layer_of(size_t tokens, size_t top_k, size_t experts, size_t hidden, size_
   return {static_cast<int>(tokens), static_cast<int>(top_k), static_cast<int>(experts), static_cast<int>(hidden), static_cast<int>(ffn)};
 }
 
-template <typename W, typename E, int MT>
+template <typename W, typename E, int MT, int FT1, int U1, int KW1, int FT2, int U2, int KW2>
 void launch(const Layer &l, const Fc1Args &a, const Fc2Args &b, E *out, hipStream_t stream) {
-  const int step = sizeof(W) == 1 ? 16 : 8;
-  const bool v1 = l.hidden % step == 0 && aligned16(a.x) && aligned16(a.w);
-  const bool v2 = l.ffn % step == 0 && aligned16(b.w);
-  hipLaunchKernelGGL((fc1_kernel<W, E, MT>), dim3(ceil_div(l.ffn, 16), l.experts), dim3(256), 0, stream, a, v1);
+  hipLaunchKernelGGL((fc1_kernel<W, E, MT, FT1, U1, KW1>), dim3(ceil_div(l.ffn, kWaves / KW1 * 16 * FT1), l.experts), dim3(256), 0, stream, a);
   NVTE_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL((fc2_kernel<W, E, MT>), dim3(ceil_div(l.hidden, 16), l.experts), dim3(256), 0, stream, b, v2);
+  hipLaunchKernelGGL((fc2_kernel<W, E, MT, FT2, U2, KW2>), dim3(ceil_div(l.hidden, kWaves / KW2 * 16 * FT2), l.experts), dim3(256), 0, stream, b);
   NVTE_CHECK_HIP(hipGetLastError());
   hipLaunchKernelGGL((combine_kernel<E>), dim3(ceil_div(l.hidden, 256), l.tokens), dim3(256), 0, stream, b.y, b.ids, out, l.top_k,
                      l.hidden, l.experts);
@@ -395,9 +541,10 @@ void launch(const Layer &l, const Fc1Args &a, const Fc2Args &b, E *out, hipStrea
 template <typename W, typename E>
 void run(const Layer &l, const Fc1Args &a, const Fc2Args &b, void *out, hipStream_t stream) {
   E *o = static_cast<E *>(out);
-  if (l.tokens <= 16) launch<W, E, 1>(l, a, b, o, stream);
-  else if (l.tokens <= 32) launch<W, E, 2>(l, a, b, o, stream);
-  else launch<W, E, 4>(l, a, b, o, stream);
+  const int per_expert = std::min(l.tokens, 2 * l.tokens * l.top_k / l.experts);
+  if (per_expert <= 16) launch<W, E, 1, 1, sizeof(W), 4, 2, sizeof(W), 4>(l, a, b, o, stream);
+  else if (per_expert <= 32) launch<W, E, 2, 2, 1, 2, 8, 1, 4>(l, a, b, o, stream);
+  else launch<W, E, 4, 2, 1, 2, 4, 1, 4>(l, a, b, o, stream);
 }
 
 }  // namespace
@@ -422,7 +569,7 @@ void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, s
       hipLaunchKernelGGL(kernel, dim3(ceil_div(tokens, 4)), dim3(256), 0, stream, logits, dtype, topk_ids, topk_weights,
                          static_cast<int64_t>(tokens), static_cast<int>(num_experts), static_cast<int>(top_k), renormalize != 0);
     };
-    if (num_experts <= 64) launch_topk(topk_kernel<1>);
+    if (num_experts <= 64) launch_topk(topk64_kernel);
     else if (num_experts <= 256) launch_topk(topk_kernel<4>);
     else launch_topk(topk_kernel<kMaxExperts / 64>);
     NVTE_CHECK_HIP(hipGetLastError());
