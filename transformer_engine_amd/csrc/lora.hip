@@ -44,21 +44,26 @@ struct ShrinkArgs {
   int features, rank, num, slice;
 };
 
-template <int MT, int RT, bool GUARD>
+template <int MT, int RT, bool GUARD, bool SMALL>
 struct ShrinkBlock {  // 64 k of every row: one 128-byte line, two operands
   u32x4 a[MT][2], b[RT][2];
-  __device__ __forceinline__ void load(const uint16_t *const (&row)[MT], const uint16_t *const (&w)[RT], int k, int end) {
+  // GUARD: the slice's ragged end, which is the row's (slices are multiples of 64)
+  __device__ __forceinline__ void load(const ShrinkArgs &p, const uint16_t *const (&row)[MT], const uint16_t *const (&w)[RT], int k,
+                                       int end) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const int at = k + 32 * h, from = GUARD ? min(at, end - 8) : at;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        if constexpr (GUARD) a[m][h] = load8_head(row[m] + k + 32 * h, end - k - 32 * h);
-        else a[m][h] = load8(row[m] + k + 32 * h);
+        if constexpr (SMALL) a[m][h] = load8_any(row[m] + at, end - at, p.in + p.tokens * p.features);
+        else if constexpr (GUARD) a[m][h] = without_head(load8(row[m] + from), at - from);
+        else a[m][h] = load8(row[m] + from);
       }
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        if constexpr (GUARD) b[j][h] = load8_head(w[j] + k + 32 * h, end - k - 32 * h);
-        else b[j][h] = load8(w[j] + k + 32 * h);
+        if constexpr (SMALL) b[j][h] = load8_any(w[j] + at, end - at, p.pool + static_cast<int64_t>(p.num) * p.rank * p.features);
+        else if constexpr (GUARD) b[j][h] = without_head(load8(w[j] + from), at - from);
+        else b[j][h] = load8(w[j] + from);
       }
     }
   }
@@ -73,8 +78,9 @@ struct ShrinkBlock {  // 64 k of every row: one 128-byte line, two operands
   }
 };
 
+// SMALL: rows of fewer than eight elements.
 // grid: token tiles x slices x phases (the tile's n-th distinct adapter is phase n % gridDim.z's); the NW waves share the slice
-template <typename E, int RT, int MT, int NW, int U>
+template <typename E, int RT, int MT, int NW, int U, bool SMALL>
 __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
   __shared__ f32x4 red[NW][MT * RT][64];
   const int lane = threadIdx.x & 63, wave = wave_index();
@@ -99,23 +105,23 @@ __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
       w[j] = p.pool + (static_cast<int64_t>(cur) * p.rank + min(j * 16 + (lane & 15), p.rank - 1)) * p.features;
     int k = first;
     for (; k + NW * 64 * (U - 1) + 64 <= end; k += NW * 64 * U) {
-      ShrinkBlock<MT, RT, false> block[U];
+      ShrinkBlock<MT, RT, false, false> block[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) block[u].load(row, w, k + u * NW * 64 + kg, end);
+      for (int u = 0; u < U; ++u) block[u].load(p, row, w, k + u * NW * 64 + kg, end);
       __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first product waits for one
 #pragma unroll
       for (int u = 0; u < U; ++u) block[u].template multiply<E>(acc);
     }
     if constexpr (U > 1) {
       for (; k + 64 <= end; k += NW * 64) {
-        ShrinkBlock<MT, RT, false> block;
-        block.load(row, w, k + kg, end);
+        ShrinkBlock<MT, RT, false, false> block;
+        block.load(p, row, w, k + kg, end);
         block.template multiply<E>(acc);
       }
     }
     if (k < end) {
-      ShrinkBlock<MT, RT, true> block;
-      block.load(row, w, k + kg, end);
+      ShrinkBlock<MT, RT, true, SMALL> block;
+      block.load(p, row, w, k + kg, end);
       block.template multiply<E>(acc);
     }
     __syncthreads();  // the last adapter's sums are read
@@ -145,9 +151,9 @@ __device__ __forceinline__ float sum_slices(const float *p, int slices, int64_t 
   for (int s0 = 0; s0 < slices; s0 += 8) {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = s0 + i < slices ? p[(s0 + i) * stride] : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = p[min(s0 + i, slices - 1) * stride];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += v[i];
+    for (int i = 0; i < 8; ++i) s += s0 + i < slices ? v[i] : 0.f;
   }
   return s;
 }
@@ -171,77 +177,137 @@ struct ExpandArgs {
 // contiguous bytes of every token.
 __device__ __forceinline__ int place(int m) { return 32 * (m & 3) + 8 * (m >> 2); }
 
-template <bool RMAJOR>
+// Ends: a chunk of eight columns past the last takes the last eight, and its lanes write only what is theirs.  Likewise the ranks:
+// `slot_rank` says which rank operand slot s stands for (-1: none, zero in the rank vector), so that the pool is always read in whole
+// eights.  A rank past the last (RMAJOR) reads the last one again and meets such a zero.
+__device__ __forceinline__ int slot_rank(int slot, int rank, bool rmajor) {
+  const int first = slot & ~7, from = rmajor || rank < 8 ? first : min(first, rank - 8), r = from + (slot & 7);
+  return r >= first && r < rank ? r : -1;
+}
+
+template <bool RMAJOR, bool SMALL>
 __device__ __forceinline__ void pool_block(const ExpandArgs &p, int adapter, int lane, int c0, int j0, u32x4 (&f)[8]) {
-  const int c = c0 + place(lane & 15), j = j0 + 8 * (lane >> 4);
+  const int c = min(c0 + place(lane & 15), max(p.features - 8, 0)), j = j0 + 8 * (lane >> 4);
   const uint16_t *w = p.pool + static_cast<int64_t>(adapter) * p.rank * p.features;
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  if constexpr (RMAJOR) {
+  const uint16_t *end = p.pool + static_cast<int64_t>(p.num) * p.rank * p.features;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = j + i < p.rank ? load8_head(w + static_cast<int64_t>(j + i) * p.features + c, p.features - c) : zero;
-    transpose8x8(f);
-  } else {
-    const uint16_t *end = p.pool + static_cast<int64_t>(p.num) * p.rank * p.features;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int valid = c + i < p.features ? p.rank - j : 0;
-      f[i] = valid > 0 ? load8_head(w + static_cast<int64_t>(c + i) * p.rank + j, valid, end) : zero;
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (RMAJOR) {
+      const uint16_t *at = w + static_cast<int64_t>(min(j + i, p.rank - 1)) * p.features + c;
+      f[i] = SMALL ? load8_any(at, p.features - c, end) : load8(at);
+    } else {
+      const uint16_t *at = w + static_cast<int64_t>(min(c + i, p.features - 1)) * p.rank + (p.rank < 8 ? j : min(j, p.rank - 8));
+      f[i] = SMALL ? load8_any(at, p.rank < 8 ? p.rank - j : 8, end) : load8(at);
     }
   }
 }
 
-template <typename E, int KT, int MT, bool RMAJOR>
-__device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, int columns, uint16_t (*s_hi)[KT * 32 + 8],
-                                            uint16_t (*s_lo)[KT * 32 + 8]) {
+// The tile's n-th distinct adapter is served by the workgroup of phase n % phases, tokens without one by phase 0.
+template <typename E, int KT, int MT, bool RMAJOR, bool SMALL>
+__device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, int columns, unsigned my_phase, unsigned phases,
+                                            uint16_t (*s_hi)[KT * 32 + 8], uint16_t (*s_lo)[KT * 32 + 8]) {
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int64_t t0 = tile * (16 * MT);
   const int id = lane < 16 * MT ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
-  const uint64_t used = __ballot(id >= 0);
-  if (used == 0 && p.base == p.out) return;
-  for (int e = threadIdx.x; e < 16 * MT * KT * 32; e += 256) {
-    const int tok = e / (KT * 32), j = e % (KT * 32);
-    float v = 0.f;
-    if (((used >> tok) & 1) && j < p.rank) {
-      const float s = p.scaling != nullptr ? p.scaling[p.ids[t0 + tok]] : 1.f;
-      v = s * sum_slices(p.low + (t0 + tok) * p.rank + j, p.slices, p.tokens * p.rank);
+  const bool without = lane < 16 * MT && t0 + lane < p.tokens && id < 0;
+  uint64_t todo = __ballot(id >= 0), write = my_phase == 0 && p.base != p.out ? __ballot(without) : 0;
+  if (phases > 1) {
+    unsigned phase = 0;
+    uint64_t left = todo;
+    todo = 0;
+    while (left != 0) {
+      const uint64_t same = __ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(left)));
+      left &= ~same;
+      if (phase++ % phases == my_phase) todo |= same;
     }
+  }
+  write |= todo;
+  if (write == 0) return;
+  const int begin = columns * p.cols, end = min(begin + p.cols, p.features);
+  // The pool's operands of the first step travel while the rank vectors are put together; later ones from the moment on that
+  // their predecessors are used up.
+  u32x4 f[KT][8];
+  auto load_pool = [&](uint64_t left, int c0) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+#pragma unroll
+    for (int k = 0; k < KT; ++k) pool_block<RMAJOR, SMALL>(p, cur, lane, c0, k * 32, f[k]);
+  };
+  int c0 = begin + wave * 128;
+  if (todo != 0 && c0 < end) load_pool(todo, c0);
+
+  const float scale = p.scaling != nullptr && id >= 0 ? p.scaling[id] : 1.f;
+  constexpr int kMine = 2 * MT * KT;  // values per thread
+  float v[kMine] = {};
+  const float *low[kMine];
+#pragma unroll
+  for (int n = 0; n < kMine; ++n) {
+    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
+    low[n] = p.low + min(t0 + tok, p.tokens - 1) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
+  }
+  const int64_t stride = p.tokens * p.rank;
+  for (int s0 = 0; s0 < p.slices; s0 += 4) {
+    float part[4][kMine];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) part[i][n] = low[n][min(s0 + i, p.slices - 1) * stride];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) v[n] += s0 + i < p.slices ? part[i][n] : 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < kMine; ++n) {
+    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
+    const float s = __shfl(scale, tok, 64);
     __bf16 h, l;
-    split1(v, h, l);
+    split1(((todo >> tok) & 1) && slot_rank(j, p.rank, RMAJOR) >= 0 ? s * v[n] : 0.f, h, l);
     s_hi[tok][j] = bits16(h);
     s_lo[tok][j] = bits16(l);
   }
-  __syncthreads();
+  // only the LDS writes have to be done: the pool's loads stay on their way
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   u32x4 hi[MT][KT], lo[MT][KT];
   int my_id[MT];
+  bool mine[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     my_id[m] = __shfl(id, m * 16 + (lane & 15), 64);
+    mine[m] = (write >> (m * 16 + (lane & 15))) & 1;
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
       hi[m][k] = *reinterpret_cast<const u32x4 *>(&s_hi[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
       lo[m][k] = *reinterpret_cast<const u32x4 *>(&s_lo[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
     }
   }
-  const int begin = columns * p.cols, end = min(begin + p.cols, p.features);
-  for (int c0 = begin + wave * 128; c0 < end; c0 += 512) {
-    // the columns' old values travel while the products run
-    u32x4 base[MT][4];
+  u32x4 base[MT][4];
+  f32x4 res[MT][8];
+  uint64_t left = todo;
+  while (c0 < end) {
+    if (left == todo) {  // a new step: the columns' old values travel while the products run
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
+        const uint16_t *from = p.base + min(t0 + m * 16 + (lane & 15), p.tokens - 1) * p.features;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t t = t0 + m * 16 + (lane & 15);
-        const int c = c0 + 32 * i + 8 * (lane >> 4);
-        base[m][i] = u32x4{0u, 0u, 0u, 0u};
-        if (p.base != nullptr && t < p.tokens) base[m][i] = load8_head(p.base + t * p.features + c, p.features - c);
+        for (int i = 0; i < 4; ++i) {
+          base[m][i] = u32x4{0u, 0u, 0u, 0u};
+          const int c = min(c0 + 32 * i + 8 * (lane >> 4), max(p.features - 8, 0));
+          if (p.base != nullptr && mine[m])
+            base[m][i] = SMALL ? load8_any(from + c, p.features - c, p.base + p.tokens * p.features) : load8(from + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) res[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-    f32x4 res[MT][8] = {};
-    for (uint64_t left = used; left != 0;) {
+    }
+    if (left != 0) {
       const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
       left &= ~__ballot(id == cur);
-      u32x4 f[KT][8];
+      if constexpr (RMAJOR) {
 #pragma unroll
-      for (int k = 0; k < KT; ++k) pool_block<RMAJOR>(p, cur, lane, c0, k * 32, f[k]);
+        for (int k = 0; k < KT; ++k) transpose8x8(f[k]);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         f32x4 acc[MT] = {};
@@ -255,40 +321,49 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
         for (int m = 0; m < MT; ++m) res[m][i] = my_id[m] == cur ? acc[m] : res[m][i];
       }
     }
+    const bool done = left == 0;
+    const int next = done ? c0 + 512 : c0;
+    if (done) left = todo;
+    if (left != 0 && next < end) load_pool(left, next);
+    if (done) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t t = t0 + m * 16 + (lane & 15);
+      for (int m = 0; m < MT; ++m) {
+        if (!mine[m]) continue;
+        uint16_t *to = p.out + (t0 + m * 16 + (lane & 15)) * p.features;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + 32 * i + 8 * (lane >> 4);
-        E o[8];
-        const E *old = reinterpret_cast<const E *>(&base[m][i]);
+        for (int i = 0; i < 4; ++i) {
+          const int c = c0 + 32 * i + 8 * (lane >> 4), first = min(c, max(p.features - 8, 0));
+          E o[8];
+          const E *old = reinterpret_cast<const E *>(&base[m][i]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) narrow(widen(old[k]) + res[m][k][i], o[k]);
-        uint16_t *to = p.out + t * p.features + c;
-        if (t < p.tokens && c + 8 <= p.features) {
-          store8(to, *reinterpret_cast<const u32x4 *>(o));
-        } else if (t < p.tokens) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (c + k < p.features) reinterpret_cast<E *>(to)[k] = o[k];
+          for (int k = 0; k < 8; ++k) narrow(widen(old[k]) + res[m][k][i], o[k]);
+          const u32x4 bits = *reinterpret_cast<const u32x4 *>(o);
+          if (c + 8 <= p.features) {
+            store8(to + c, bits);
+          } else if (c < p.features) {
+            uint64_t half[2] = {bits[0] | static_cast<uint64_t>(bits[1]) << 32, bits[2] | static_cast<uint64_t>(bits[3]) << 32};
+#pragma unroll 1
+            for (int k = c - first; k < min(8, p.features - first); ++k)
+              to[first + k] = static_cast<uint16_t>((k < 4 ? half[0] : half[1]) >> (16 * (k & 3)));
+          }
         }
       }
     }
+    c0 = next;
   }
 }
 
-// grid: token tiles x column ranges
-template <typename E, int KT, int MT, bool RMAJOR>
+// grid: token tiles x column ranges x phases
+template <typename E, int KT, int MT, bool SMALL>
 __global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p) {
   // 16-byte aligned rows, neighbouring rows in different banks
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
-  expand_tile<E, KT, MT, RMAJOR>(p, blockIdx.x, blockIdx.y, s_hi, s_lo);
+  expand_tile<E, KT, MT, false, SMALL>(p, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, s_hi, s_lo);
 }
 
 // ====================================================================================
-// prepare: the tokens of every adapter in rising order, each adapter's list padded to whole blocks of 32 with -1; where they
-// begin; where its work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to [rank][features].
+// prepare: the tokens of every adapter in rising order, each adapter's list padded to whole blocks of 32 with its last token, marked
+// by the sign bit; where they begin; where its work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to [rank][features].
 // One workgroup per adapter counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged; its sixteen waves own
 // consecutive stretches of the tokens.
 // ====================================================================================
@@ -366,10 +441,12 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   for (int64_t t0 = from; t0 < to; t0 += 64) {
     const bool hit = t0 + lane < to && p.ids[t0 + lane] == a;
     const uint64_t m = __ballot(hit);
-    if (hit) order[at + __popcll(m & ((1ull << lane) - 1))] = static_cast<int>(t0) + lane;
+    const int to_slot = at + __popcll(m & ((1ull << lane) - 1)), t = static_cast<int>(t0) + lane;
+    if (hit) order[to_slot] = t;
+    if (hit && to_slot == mine - 1)
+      for (int i = mine; i < my_blocks * kBlock; ++i) order[i] = t | INT_MIN;
     at += __popcll(m);
   }
-  if (threadIdx.x < my_blocks * kBlock - mine) order[mine + threadIdx.x] = -1;
 }
 
 // 64 features of one adapter's matrix
@@ -432,10 +509,9 @@ __device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &si
   for (int e = threadIdx.x; e < kBlock * tiles * 16; e += 256) {
     const int j = e % (tiles * 16), tok = e / (tiles * 16);
     const int t = p.plan.order[block * kBlock + tok];
-    float v = 0.f;
-    if (t >= 0 && j < p.rank) v = scale * sum_slices(side.low + static_cast<int64_t>(t) * p.rank + j, side.slices, p.tokens * p.rank);
+    const float s = sum_slices(side.low + static_cast<int64_t>(t & INT_MAX) * p.rank + min(j, p.rank - 1), side.slices, p.tokens * p.rank);
     __bf16 h, l;
-    split1(v, h, l);
+    split1(t >= 0 && j < p.rank ? scale * s : 0.f, h, l);
     const int at = (j >> 4) * 1024 + ((j & 15) + 16 * (tok >> 3)) * 8 + (tok & 7);
     out[at] = bits16(h);
     out[at + 512] = bits16(l);
@@ -443,127 +519,150 @@ __device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &si
 }
 
 // the backward pass's `expand` and `pack` read the same rank vectors and nothing of each other: one launch
-template <typename E, int KT, int MT>
-__global__ __launch_bounds__(256) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int blocks) {
+template <typename E, int KT, int MT, bool SMALL>
+__global__ __launch_bounds__(256) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int phases,
+                                                          int blocks) {
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
   const int b = blockIdx.x;
   if (b < 2 * blocks) pack_block(q, b < blocks ? q.side[0] : q.side[1], b < blocks ? b : b - blocks);
-  else expand_tile<E, KT, MT, true>(p, (b - 2 * blocks) % tiles, (b - 2 * blocks) / tiles, s_hi, s_lo);
+  else {
+    const int n = (b - 2 * blocks) / tiles;
+    expand_tile<E, KT, MT, true, SMALL>(p, (b - 2 * blocks) % tiles, n % column_ranges, n / column_ranges, phases, s_hi, s_lo);
+  }
 }
 
 // ====================================================================================
-// wgrad: one work item's dA [r][K] = sum_t w[t] (x) x[t] and dB [O][r] = sum_t dy[t] (x) w[t]
+// wgrad: one work item's sums over its tokens of w[t] (x) z[t]: dA with z = x, dB (transposed) with z = dy
 // ====================================================================================
 struct WgradSide {
   const uint16_t *z;       // activations [tokens][features]
   const uint16_t *packed;  // rank vectors
-  void *grad;              // [num][rank][features] or [num][features][rank]
-  float *part;             // per item, the same layout in fp32
+  float *part;             // [item][rank][features]
+  void *grad;              // [num][rank][features], or [num][features][rank] (the second side)
   int features, groups;    // groups: workgroups along the features, 512 columns each
 };
 struct WgradArgs {
-  WgradSide a, b;
+  WgradSide side[2];
   Plan plan;
+  int64_t tokens;
   int rank, num, per_item, grad_type;
 };
 
-template <typename E, int RT>
-struct WgradBlock {  // 32 tokens x 128 columns, and their rank vectors
+struct WgradTokens {  // a lane's eight tokens of a block
+  int t[8];
+  __device__ __forceinline__ void load(const int *order, int block, int lane) {
+    const int *from = order + static_cast<int64_t>(block) * kBlock + 8 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from[i];
+  }
+};
+
+template <typename E, int RT, bool SMALL>
+struct WgradBlock {  // 32 tokens x 128 columns, and their rank vectors (zero for padding, whose rows are the adapter's own)
   u32x4 z[8], w[RT][2];
-  __device__ __forceinline__ void load(const WgradSide &side, const int *order, int64_t block, int rank_tiles, int j0, int c, int lane) {
-    const int *tokens = order + block * kBlock + 8 * (lane >> 4);
-    const uint16_t *w0 = side.packed + (block * rank_tiles + j0) * 1024 + lane * 8;
+  __device__ __forceinline__ void load(const WgradSide &side, int64_t all, const WgradTokens &tokens, int block, int rank_tiles,
+                                       int j0, int c, int lane) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int t = tokens[i];
-      z[i] = u32x4{0u, 0u, 0u, 0u};
-      if (t >= 0) z[i] = load8_head(side.z + static_cast<int64_t>(t) * side.features + c, side.features - c);
+      const uint16_t *at = side.z + static_cast<int64_t>(tokens.t[i] & INT_MAX) * side.features + c;
+      z[i] = SMALL ? load8_any(at, side.features - c, side.z + all * side.features) : load8(at);
     }
+    const uint16_t *from = side.packed + (static_cast<int64_t>(block) * rank_tiles + j0) * 1024 + lane * 8;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
-      w[j][0] = *reinterpret_cast<const u32x4 *>(w0 + min(j, rank_tiles - j0 - 1) * 1024);
-      w[j][1] = *reinterpret_cast<const u32x4 *>(w0 + min(j, rank_tiles - j0 - 1) * 1024 + 512);
+      w[j][0] = *reinterpret_cast<const u32x4 *>(from + min(j, rank_tiles - j0 - 1) * 1024);
+      w[j][1] = *reinterpret_cast<const u32x4 *>(from + min(j, rank_tiles - j0 - 1) * 1024 + 512);
     }
   }
-  template <bool IS_B>
   __device__ __forceinline__ void multiply(f32x4 (&acc)[RT][8]) {
     transpose8x8(z);
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
       const Terms<E> terms(z[f]);
 #pragma unroll
-      for (int j = 0; j < RT; ++j) acc[j][f] = mfma16_split<E, !IS_B>(terms, w[j][0], w[j][1], acc[j][f]);
+      for (int j = 0; j < RT; ++j) acc[j][f] = mfma16_split<E, true>(terms, w[j][0], w[j][1], acc[j][f]);
     }
   }
 };
 
-template <typename E, int RT, bool IS_B>
-__device__ __forceinline__ void wgrad_side(const WgradArgs &p, const WgradSide &side, int group) {
+// grid: column groups of both sides  x  work items (an upper bound; the rest leave at once)  x  64 ranks
+template <typename E, int RT, bool SMALL>
+__global__ __launch_bounds__(256, RT <= 2 ? 2 : 1) void wgrad_kernel(WgradArgs p) {
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int item = blockIdx.y;
   if (item >= p.plan.item_base[p.num]) return;
+  const bool second = static_cast<int>(blockIdx.x) >= p.side[0].groups;
+  const WgradSide side = second ? p.side[1] : p.side[0];
+  const int c0 = (blockIdx.x - (second ? p.side[0].groups : 0)) * 512 + wave * 128;
+  if (c0 >= side.features) return;
   const int a = __builtin_amdgcn_readfirstlane(owner_of(p.plan.item_base, p.num, item));
   const int first = __builtin_amdgcn_readfirstlane(p.plan.block_base[a] + (item - p.plan.item_base[a]) * p.per_item);
   const int last = __builtin_amdgcn_readfirstlane(min(first + p.per_item, p.plan.block_base[a + 1]));
-  const bool whole = p.plan.item_base[a + 1] - p.plan.item_base[a] == 1;
-  const int c0 = group * 512 + wave * 128, c = c0 + 8 * (lane & 15);
-  if (c0 >= side.features) return;
+  // a lane past the last column computes the last eight once more, and stores the same values
+  const int c = min(c0 + 8 * (lane & 15), max(side.features - 8, 0));
   const int rank_tiles = (p.rank + 15) / 16, j0 = blockIdx.z * 4;
+  const int *order = p.plan.order;
   f32x4 acc[RT][8] = {};
-  // the next block is on its way while the products of this one run
-  WgradBlock<E, RT> even, odd;
-  even.load(side, p.plan.order, first, rank_tiles, j0, c, lane);
+  // while the products of one block run, the next block is on its way, and the one after's token numbers
+  WgradTokens t0, t1;
+  WgradBlock<E, RT, SMALL> even, odd;
+  t0.load(order, first, lane);
+  t1.load(order, min(first + 1, last - 1), lane);
+  even.load(side, p.tokens, t0, first, rank_tiles, j0, c, lane);
   for (int b = first;;) {
-    odd.load(side, p.plan.order, min(b + 1, last - 1), rank_tiles, j0, c, lane);
+    t0.load(order, min(b + 2, last - 1), lane);
+    odd.load(side, p.tokens, t1, min(b + 1, last - 1), rank_tiles, j0, c, lane);
     __builtin_amdgcn_sched_barrier(0);
-    even.template multiply<IS_B>(acc);
+    even.multiply(acc);
     if (++b >= last) break;
-    even.load(side, p.plan.order, min(b + 1, last - 1), rank_tiles, j0, c, lane);
+    t1.load(order, min(b + 2, last - 1), lane);
+    even.load(side, p.tokens, t0, min(b + 1, last - 1), rank_tiles, j0, c, lane);
     __builtin_amdgcn_sched_barrier(0);
-    odd.template multiply<IS_B>(acc);
+    odd.multiply(acc);
     if (++b >= last) break;
   }
-  const int64_t size = static_cast<int64_t>(p.rank) * side.features;
-  const int64_t base = (whole ? a : item) * size;
-  void *out = whole ? side.grad : side.part;
-  const int type = whole ? p.grad_type : kNVTEFloat32;
-  const int r0 = j0 * 16;
+  float *out = side.part + static_cast<int64_t>(item) * p.rank * side.features + c;
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
   for (int j = 0; j < RT; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const int row = (j0 + j) * 16 + (lane >> 4) * 4 + i;
+      if (row >= p.rank) continue;
+      float *to = out + static_cast<int64_t>(row) * side.features;
+      if (!SMALL || side.features >= 8) {
+        *reinterpret_cast<f32x4_any *>(to) = f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
+        *reinterpret_cast<f32x4_any *>(to + 4) = f32x4{acc[j][4][i], acc[j][5][i], acc[j][6][i], acc[j][7][i]};
+      } else {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        if constexpr (IS_B) {  // rows are features, columns ranks
-          const int row = c0 + 8 * (4 * (lane >> 4) + i) + f, col = r0 + j * 16 + (lane & 15);
-          if (row < side.features && col < p.rank) store1(out, base + static_cast<int64_t>(row) * p.rank + col, type, acc[j][f][i]);
-        } else {
-          const int row = r0 + j * 16 + (lane >> 4) * 4 + i, col = c + f;
-          if (row < p.rank && col < side.features) store1(out, base + static_cast<int64_t>(row) * side.features + col, type, acc[j][f][i]);
-        }
+        for (int f = 0; f < 7; ++f)
+          if (f < side.features) to[f] = acc[j][f][i];
       }
+    }
 }
 
-// grid: column groups of dA, then of dB  x  work items (an upper bound; the rest leave at once)  x  64 ranks
-template <typename E, int RT>
-__global__ __launch_bounds__(256) void wgrad_kernel(WgradArgs p) {
-  const int group = blockIdx.x;
-  if (group < p.a.groups) wgrad_side<E, RT, false>(p, p.a, group);
-  else wgrad_side<E, RT, true>(p, p.b, group - p.a.groups);
-}
-
-// join: the sum of an adapter's work items in their order; zero for an adapter without tokens.  grid: elements x adapters
-__global__ __launch_bounds__(256) void join_kernel(WgradArgs p) {
+// join: the sum of an adapter's work items in their order; zero for an adapter without tokens.  A workgroup takes 64 columns of
+// all ranks: dA is written as it is read, dB turned round in LDS.  grid: column pieces of both sides x adapters
+__global__ __launch_bounds__(256) void join_kernel(WgradArgs p, int pieces) {
+  __shared__ float s[64 * (kMaxRank + 1)];
   const int a = blockIdx.y;
+  const bool second = static_cast<int>(blockIdx.x) >= pieces;
+  const WgradSide side = second ? p.side[1] : p.side[0];
+  const int c0 = (blockIdx.x - (second ? pieces : 0)) * 64, columns = min(64, side.features - c0);
   const int first = p.plan.item_base[a], items = p.plan.item_base[a + 1] - first;
-  if (items == 1) return;
-  const int64_t size_a = static_cast<int64_t>(p.rank) * p.a.features, size_b = static_cast<int64_t>(p.rank) * p.b.features;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < size_a + size_b; e += gridDim.x * 256ll) {
-    const bool is_a = e < size_a;
-    const float *part = is_a ? p.a.part : p.b.part;
-    const int64_t at = is_a ? e : e - size_a, size = is_a ? size_a : size_b;
-    store1(is_a ? p.a.grad : p.b.grad, a * size + at, p.grad_type, sum_slices(part + first * size + at, items, size));
+  const int64_t size = static_cast<int64_t>(p.rank) * side.features;
+  const int lane = threadIdx.x & 63;
+  for (int j = threadIdx.x >> 6; j < p.rank; j += 4) {
+    if (lane >= columns) continue;
+    const int64_t at = static_cast<int64_t>(j) * side.features + c0 + lane;
+    const float v = items > 0 ? sum_slices(side.part + first * size + at, items, size) : 0.f;
+    if (second) s[lane * (p.rank + 1) + j] = v;
+    else store1(side.grad, a * size + at, p.grad_type, v);
   }
+  if (!second) return;
+  __syncthreads();
+  for (int e = threadIdx.x; e < columns * p.rank; e += 256)
+    store1(side.grad, a * size + static_cast<int64_t>(c0) * p.rank + e, p.grad_type, s[e / p.rank * (p.rank + 1) + e % p.rank]);
 }
 
 // ====================================================================================
@@ -597,13 +696,17 @@ int slice_of(int64_t tokens, int features) {
 }
 int num_slices(int64_t tokens, int features) { return static_cast<int>(ceil_div(features, slice_of(tokens, features))); }
 
-template <typename E, int RT, int MT, int NW, int U>
+// a decode tile's adapters go to workgroups of their own while there are too few of them
+int phases_of(int64_t workgroups, int64_t tokens, int num) {
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(num, tokens), 16);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 2048 / workgroups)));
+}
+
+template <typename E, int RT, int MT, int NW, int U, bool SMALL = false>
 void launch_shrink(const ShrinkArgs &p, int slices, hipStream_t stream) {
   const int64_t tiles = (p.tokens + 16 * MT - 1) / (16 * MT);
-  // a decode tile's adapters go to workgroups of their own while there are too few tiles
-  const int64_t most = std::min<int64_t>(std::min<int64_t>(p.num, p.tokens), 16);
-  const int64_t phases = std::max<int64_t>(1, std::min<int64_t>(most, 2048 / (tiles * slices)));
-  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, U>), dim3(tiles, slices, phases), dim3(NW * 64), 0, stream, p);
+  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, U, SMALL>), dim3(tiles, slices, phases_of(tiles * slices, p.tokens, p.num)),
+                     dim3(NW * 64), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
@@ -614,7 +717,9 @@ void shrink(const void *in, const void *pool, const int *ids, float *out, int64_
                      slice_of(tokens, features)};
   const int slices = num_slices(tokens, features);
   const bool many = many_tokens(tokens);
-  if (rank <= 16) {
+  if (features < 8) {
+    launch_shrink<E, 8, 1, 4, 1, true>(p, slices, stream);
+  } else if (rank <= 16) {
     many ? launch_shrink<E, 1, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 1, 1, 4, 2>(p, slices, stream);
   } else if (rank <= 32) {
     many ? launch_shrink<E, 2, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 2, 1, 4, 2>(p, slices, stream);
@@ -625,16 +730,18 @@ void shrink(const void *in, const void *pool, const int *ids, float *out, int64_
   }
 }
 
-// runs launch(KT, MT) as integral constants: 32 ranks per operand, 16 tokens per tile
+// runs launch(KT, MT, SMALL) as integral constants: 32 ranks per operand, 16 tokens per tile
 template <typename Launch>
-void expand_variant(int rank, int64_t tokens, Launch &&launch) {
+void expand_variant(int rank, int64_t tokens, bool small_features, bool small_rank, Launch &&launch) {
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
   typedef std::integral_constant<int, 4> Four;
   const bool many = tokens >= 1024;
-  if (rank <= 32) many ? launch(One(), Two()) : launch(One(), One());
-  else if (rank <= 64) many ? launch(Two(), Two()) : launch(Two(), One());
-  else launch(Four(), One());
+  if (small_features) launch(Four(), One(), std::true_type());
+  else if (small_rank) many ? launch(One(), Two(), std::true_type()) : launch(One(), One(), std::true_type());
+  else if (rank <= 32) many ? launch(One(), Two(), std::false_type()) : launch(One(), One(), std::false_type());
+  else if (rank <= 64) many ? launch(Two(), Two(), std::false_type()) : launch(Two(), One(), std::false_type());
+  else launch(Four(), One(), std::false_type());
 }
 
 // columns per workgroup: 512 until there are about 2048 workgroups
@@ -645,34 +752,39 @@ int columns_of(int64_t tiles, int features) {
 
 template <typename E>
 void expand(ExpandArgs p, hipStream_t stream) {
-  expand_variant(p.rank, p.tokens, [&](auto kt, auto mt) {
+  expand_variant(p.rank, p.tokens, p.features < 8, p.rank < 8, [&](auto kt, auto mt, auto small) {
     const int64_t tiles = ceil_div(p.tokens, 16 * mt());
     p.cols = columns_of(tiles, p.features);
-    hipLaunchKernelGGL((expand_kernel<E, kt(), mt(), false>), dim3(tiles, ceil_div(p.features, p.cols)), dim3(256), 0, stream, p);
+    const int64_t ranges = ceil_div(p.features, p.cols);
+    hipLaunchKernelGGL((expand_kernel<E, kt(), mt(), small()>), dim3(tiles, ranges, phases_of(tiles * ranges, p.tokens, p.num)),
+                       dim3(256), 0, stream, p);
     NVTE_CHECK_HIP(hipGetLastError());
   });
 }
 
 template <typename E>
 void expand_and_pack(ExpandArgs p, const PackArgs &q, int64_t blocks, hipStream_t stream) {
-  expand_variant(p.rank, p.tokens, [&](auto kt, auto mt) {
+  expand_variant(p.rank, p.tokens, p.features < 8, false, [&](auto kt, auto mt, auto small) {
     const int64_t tiles = ceil_div(p.tokens, 16 * mt());
     p.cols = columns_of(tiles, p.features);
-    const int64_t ranges = p.out != nullptr ? ceil_div(p.features, p.cols) : 0, grid = 2 * blocks + tiles * ranges;
+    const int64_t ranges = p.out != nullptr ? ceil_div(p.features, p.cols) : 0;
+    const int phases = phases_of(std::max<int64_t>(1, tiles * ranges), p.tokens, p.num);
+    const int64_t grid = 2 * blocks + tiles * ranges * phases;
     NVTE_CHECK(grid <= INT_MAX, "too many workgroups: ", grid);
     if (grid == 0) return;
-    hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt()>), dim3(grid), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
-                       static_cast<int>(tiles), static_cast<int>(blocks));
+    hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt(), small()>), dim3(grid), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
+                       static_cast<int>(tiles), phases, static_cast<int>(blocks));
     NVTE_CHECK_HIP(hipGetLastError());
   });
 }
 
 template <typename E>
 void launch_wgrad(const WgradArgs &p, unsigned items, hipStream_t stream) {
-  const dim3 grid(p.a.groups + p.b.groups, items, ceil_div(p.rank, 64));
-  if (p.rank <= 16) hipLaunchKernelGGL((wgrad_kernel<E, 1>), grid, dim3(256), 0, stream, p);
-  else if (p.rank <= 32) hipLaunchKernelGGL((wgrad_kernel<E, 2>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((wgrad_kernel<E, 4>), grid, dim3(256), 0, stream, p);
+  const dim3 grid(p.side[0].groups + p.side[1].groups, items, ceil_div(p.rank, 64));
+  if (p.side[0].features < 8 || p.side[1].features < 8) hipLaunchKernelGGL((wgrad_kernel<E, 4, true>), grid, dim3(256), 0, stream, p);
+  else if (p.rank <= 16) hipLaunchKernelGGL((wgrad_kernel<E, 1, false>), grid, dim3(256), 0, stream, p);
+  else if (p.rank <= 32) hipLaunchKernelGGL((wgrad_kernel<E, 2, false>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((wgrad_kernel<E, 4, false>), grid, dim3(256), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
@@ -739,11 +851,12 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   }
   if (!wgrad) return;
   WgradArgs p{};
-  p.a = {static_cast<const uint16_t *>(x), packed_a, da, reinterpret_cast<float *>(ws + w.part_a), s.in,
-         static_cast<int>(ceil_div(s.in, 512))};
-  p.b = {static_cast<const uint16_t *>(dy), packed_b, db, reinterpret_cast<float *>(ws + w.part_b), s.out,
-         static_cast<int>(ceil_div(s.out, 512))};
+  p.side[0] = {static_cast<const uint16_t *>(x), packed_a, reinterpret_cast<float *>(ws + w.part_a), da, s.in,
+               static_cast<int>(ceil_div(s.in, 512))};
+  p.side[1] = {static_cast<const uint16_t *>(dy), packed_b, reinterpret_cast<float *>(ws + w.part_b), db, s.out,
+               static_cast<int>(ceil_div(s.out, 512))};
   p.plan = plan;
+  p.tokens = s.tokens;
   p.rank = s.rank;
   p.num = s.num;
   p.per_item = per_item;
@@ -751,9 +864,8 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   const int64_t items = most_items(s);
   NVTE_CHECK(items <= 65535, "too many work items: ", items);
   if (items > 0) launch_wgrad<E>(p, static_cast<unsigned>(items), stream);
-  const int64_t elements = static_cast<int64_t>(s.rank) * (static_cast<int64_t>(s.in) + s.out);
-  const int64_t grid = std::min<int64_t>(ceil_div(elements, 256), std::max<int64_t>(1, 4096 / s.num));
-  hipLaunchKernelGGL(join_kernel, dim3(grid, s.num), dim3(256), 0, stream, p);
+  const int columns = static_cast<int>(ceil_div(s.in, 64));
+  hipLaunchKernelGGL(join_kernel, dim3(columns + ceil_div(s.out, 64), s.num), dim3(256), 0, stream, p, columns);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 

@@ -89,21 +89,33 @@ __device__ __forceinline__ f32x4 mfma16_split(const Terms<E> &w, u32x4 hi, u32x4
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ u32x4 load8(const uint16_t *p) { return *reinterpret_cast<const u32x4_any *>(p); }
 __device__ __forceinline__ void store8(uint16_t *p, u32x4 v) { *reinterpret_cast<u32x4_any *>(p) = v; }
-// the first `valid` of them, zeros after; nothing behind p + valid is touched
-__device__ __forceinline__ u32x4 load8_head(const uint16_t *p, int valid) {
-  if (valid >= 8) return load8(p);
-  u32x4 v = {0u, 0u, 0u, 0u};
+// The ends of rows whose length is no multiple of the step: a lane whose eight elements would reach past the end takes the last
+// eight instead and, where they are summed, has the `skip` that its neighbour holds already set to zero.  This keeps the kernels
+// small (instruction cache misses cost these short kernels more than the arithmetic: an expand kernel with element-wise ends had 32 KiB
+// of code and ran 18 us on 6 MB).
+__device__ __forceinline__ u32x4 without_head(u32x4 v, int skip) {
 #pragma unroll
-  for (int i = 0; i < 7; ++i)
-    if (i < valid) v[i >> 1] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
+  for (int w = 0; w < 4; ++w) v[w] &= skip <= 2 * w ? 0xFFFFFFFFu : skip <= 2 * w + 1 ? 0xFFFF0000u : 0u;
   return v;
 }
-// the same where p + 8 may reach into memory of the same array that ends at `end`: one access and a mask away from its end
-__device__ __forceinline__ u32x4 load8_head(const uint16_t *p, int valid, const uint16_t *end) {
-  if (valid >= 8 || p + 8 > end) return load8_head(p, valid);
-  u32x4 v = load8(p);
+// Rows of fewer elements than a step (kernel variants of their own, SMALL): the first n, zeros after.  p .. end belongs to one array, so
+// away from its end one access and a mask do.
+__device__ __forceinline__ u32x4 load8_any(const uint16_t *p, int n, const uint16_t *end) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n > 0 && p + 8 <= end) {
+    v = load8(p);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) v[w] &= valid > 2 * w + 1 ? 0xFFFFFFFFu : valid > 2 * w ? 0xFFFFu : 0u;
+    for (int w = 0; w < 4; ++w) v[w] &= n > 2 * w + 1 ? 0xFFFFFFFFu : n > 2 * w ? 0xFFFFu : 0u;
+  } else {
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int i = 0; i < min(n, 8); ++i) {
+      const uint64_t x = p[i];
+      if (i < 4) lo |= x << (16 * i);
+      else hi |= x << (16 * (i - 4));
+    }
+    v = u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32)};
+  }
   return v;
 }
 

@@ -152,9 +152,9 @@ struct Line<uint16_t> {
     v[0] = load8(p);
     v[1] = load8(p + 8);
   }
-  __device__ __forceinline__ void load_head(const uint16_t *p, int valid) {
-    v[0] = load8_head(p, valid);
-    v[1] = load8_head(p + 8, valid - 8);
+  __device__ __forceinline__ void load_any(const uint16_t *p, int n, const uint16_t *end) {
+    v[0] = load8_any(p, n, end);
+    v[1] = load8_any(p + 8, n - 8, end);
   }
   template <typename E>
   __device__ __forceinline__ u32x4 operand(int i) const {
@@ -171,15 +171,12 @@ struct Line<fp8_t> {
     v[0] = *reinterpret_cast<const any *>(p);
     v[1] = *reinterpret_cast<const any *>(p + 16);
   }
-  __device__ __forceinline__ void load_head(const fp8_t *p, int valid) {
-    if (valid >= 32) return load(p);
+  __device__ __forceinline__ void load_any(const fp8_t *p, int n, const fp8_t *) {
+    v[0] = v[1] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      uint32_t d = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * w + i < valid) d |= static_cast<uint32_t>(p[4 * w + i].bits) << (8 * i);
-      v[w >> 2][w & 3] = d;
+#pragma unroll 1
+      for (int i = 0; i < min(n - 4 * w, 4); ++i) v[w >> 2][w & 3] |= static_cast<uint32_t>(p[4 * w + i].bits) << (8 * i);
     }
   }
   template <typename E>
@@ -239,14 +236,16 @@ struct Fc1Args {
   const float *scale_inv;  // [experts], null: 1
   const int *ids;          // [tokens][top_k]
   uint16_t *h_hi, *h_lo;   // [pairs][ffn]
-  int pairs, top_k, hidden, ffn;
+  int pairs, top_k, experts, hidden, ffn;
 };
 
-template <typename W, typename E, int MT, int FT, int KW>
+template <typename W, typename E, int MT, int FT, int KW, bool SMALL>
 struct Fc1 {
   const W *gate[FT];        // this lane's rows of the gate half
   int64_t up;               // from there to the other half's
   const uint16_t *row[MT];  // this lane's tokens
+  const W *w_end;           // ends of the arrays (SMALL)
+  const uint16_t *x_end;
   int hidden, lane;
 
   template <int U, bool GUARD>
@@ -255,15 +254,17 @@ struct Fc1 {
     static constexpr int N = L::kOps;
     L g[U][FT], u[U][FT];
     u32x4 x[U][MT][N];
+    // SMALL: rows of fewer than 8 N elements.  GUARD: the row's ragged end.  A lane past it takes the last 8 N elements (see mfma16.h); x alone is cleared of what
+    // other lanes hold.
     __device__ __forceinline__ void load(const Fc1 &p, int block) {
 #pragma unroll
       for (int s = 0; s < U; ++s) {
-        const int k = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N);
+        const int at = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N), k = GUARD ? min(at, p.hidden - 8 * N) : at;
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
-          if constexpr (GUARD) {
-            g[s][f].load_head(p.gate[f] + k, p.hidden - k);
-            u[s][f].load_head(p.gate[f] + p.up + k, p.hidden - k);
+          if constexpr (SMALL) {
+            g[s][f].load_any(p.gate[f] + at, p.hidden - at, p.w_end);
+            u[s][f].load_any(p.gate[f] + p.up + at, p.hidden - at, p.w_end);
           } else {
             g[s][f].load(p.gate[f] + k);
             u[s][f].load(p.gate[f] + p.up + k);
@@ -273,8 +274,9 @@ struct Fc1 {
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int o = 0; o < N; ++o) {
-            if constexpr (GUARD) x[s][m][o] = load8_head(p.row[m] + k + 8 * o, p.hidden - k - 8 * o);
+            if constexpr (SMALL) x[s][m][o] = load8_any(p.row[m] + at + 8 * o, p.hidden - at - 8 * o, p.x_end);
             else x[s][m][o] = load8(p.row[m] + k + 8 * o);
+            if constexpr (GUARD && !SMALL) x[s][m][o] = without_head(x[s][m][o], at - k - 8 * o);
           }
       }
     }
@@ -319,7 +321,7 @@ __device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*red)[64], in
 }
 
 // grid: (4 / KW) 16 FT rows of the gate half (and the same of the other) x experts
-template <typename W, typename E, int MT, int FT, int U, int KW>
+template <typename W, typename E, int MT, int FT, int U, int KW, bool SMALL>
 __global__ __launch_bounds__(256) void fc1_kernel(Fc1Args p) {
   __shared__ uint16_t list[kMaxPairs];
   __shared__ int scratch[kWaves];
@@ -329,11 +331,13 @@ __global__ __launch_bounds__(256) void fc1_kernel(Fc1Args p) {
   const int n = __builtin_amdgcn_readfirstlane(find_pairs(p.ids, p.pairs, e, list, scratch));
   if (n == 0) return;
   const W *w = static_cast<const W *>(p.w) + static_cast<int64_t>(e) * 2 * p.ffn * p.hidden;
-  typedef Fc1<W, E, MT, FT, KW> Side;
+  typedef Fc1<W, E, MT, FT, KW, SMALL> Side;
   Side side;
   side.up = static_cast<int64_t>(p.ffn) * p.hidden;
   side.hidden = p.hidden;
   side.lane = lane;
+  side.w_end = static_cast<const W *>(p.w) + static_cast<int64_t>(p.experts) * 2 * p.ffn * p.hidden;
+  side.x_end = static_cast<const uint16_t *>(p.x) + static_cast<int64_t>(p.pairs / p.top_k) * p.hidden;
 #pragma unroll
   for (int f = 0; f < FT; ++f) side.gate[f] = w + static_cast<int64_t>(min(f0 + f * 16 + (lane & 15), p.ffn - 1)) * p.hidden;
   const float scale = p.scale_inv != nullptr ? p.scale_inv[e] : 1.f;
@@ -381,7 +385,7 @@ struct Fc2Args {
   const int *ids;               // [tokens][top_k]
   const float *weights;         // [tokens][top_k]
   float *y;                     // [pairs][hidden]
-  int pairs, hidden, ffn;
+  int pairs, experts, hidden, ffn;
 };
 
 // the format in which stored weights meet h's bf16 terms: FP8 is widened (exact), 16-bit types stay
@@ -394,11 +398,13 @@ struct Fc2Type<fp8_t, E> {
   typedef bf16_t type;
 };
 
-template <typename W, typename E, int MT, int FT, int KW>
+template <typename W, typename E, int MT, int FT, int KW, bool SMALL>
 struct Fc2 {
   const W *w[FT];                // this lane's rows
   const uint16_t *hi[MT];        // this lane's tokens
   int64_t lo;                    // from hi to their second terms
+  const W *w_end;                // ends of the arrays (SMALL)
+  const uint16_t *h_end;
   int ffn, lane;
 
   template <int U, bool GUARD>
@@ -411,10 +417,10 @@ struct Fc2 {
     __device__ __forceinline__ void load(const Fc2 &p, int block) {
 #pragma unroll
       for (int s = 0; s < U; ++s) {
-        const int k = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N);
+        const int at = (block + s * KW) * L::kBlock + (p.lane >> 4) * (8 * N), k = GUARD ? min(at, p.ffn - 8 * N) : at;
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
-          if constexpr (GUARD) r[s][f].load_head(p.w[f] + k, p.ffn - k);
+          if constexpr (SMALL) r[s][f].load_any(p.w[f] + at, p.ffn - at, p.w_end);
           else r[s][f].load(p.w[f] + k);
         }
 #pragma unroll
@@ -423,9 +429,10 @@ struct Fc2 {
           for (int o = 0; o < N; ++o)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const uint16_t *at = p.hi[m] + t * p.lo + k + 8 * o;
-              if constexpr (GUARD) h[s][m][o][t] = load8_head(at, p.ffn - k - 8 * o);
-              else h[s][m][o][t] = load8(at);
+              const uint16_t *from = p.hi[m] + t * p.lo;
+              if constexpr (SMALL) h[s][m][o][t] = load8_any(from + at + 8 * o, p.ffn - at - 8 * o, p.h_end);
+              else h[s][m][o][t] = load8(from + k + 8 * o);
+              if constexpr (GUARD && !SMALL) h[s][m][o][t] = without_head(h[s][m][o][t], at - k - 8 * o);
             }
       }
     }
@@ -446,7 +453,7 @@ struct Fc2 {
 };
 
 // grid: (4 / KW) 16 FT rows of the output x experts
-template <typename W, typename E, int MT, int FT, int U, int KW>
+template <typename W, typename E, int MT, int FT, int U, int KW, bool SMALL>
 __global__ __launch_bounds__(256) void fc2_kernel(Fc2Args p) {
   __shared__ uint16_t list[kMaxPairs];
   __shared__ int scratch[kWaves];
@@ -455,11 +462,13 @@ __global__ __launch_bounds__(256) void fc2_kernel(Fc2Args p) {
   const int e = blockIdx.y, c0 = (blockIdx.x * (kWaves / KW) + wave / KW) * (16 * FT);
   const int n = __builtin_amdgcn_readfirstlane(find_pairs(p.ids, p.pairs, e, list, scratch));
   if (n == 0) return;
-  typedef Fc2<W, E, MT, FT, KW> Side;
+  typedef Fc2<W, E, MT, FT, KW, SMALL> Side;
   Side side;
   side.lo = p.h_lo - p.h_hi;
   side.ffn = p.ffn;
   side.lane = lane;
+  side.w_end = static_cast<const W *>(p.w) + static_cast<int64_t>(p.experts) * p.hidden * p.ffn;
+  side.h_end = p.h_hi + 2 * side.lo;
 #pragma unroll
   for (int f = 0; f < FT; ++f)
     side.w[f] = static_cast<const W *>(p.w) + (static_cast<int64_t>(e) * p.hidden + min(c0 + f * 16 + (lane & 15), p.hidden - 1)) * p.ffn;
@@ -529,9 +538,14 @@ Layer layer_of(size_t tokens, size_t top_k, size_t experts, size_t hidden, size_
 
 template <typename W, typename E, int MT, int FT1, int U1, int KW1, int FT2, int U2, int KW2>
 void launch(const Layer &l, const Fc1Args &a, const Fc2Args &b, E *out, hipStream_t stream) {
-  hipLaunchKernelGGL((fc1_kernel<W, E, MT, FT1, U1, KW1>), dim3(ceil_div(l.ffn, kWaves / KW1 * 16 * FT1), l.experts), dim3(256), 0, stream, a);
+  constexpr int kShort = 8 * Line<W>::kOps;
+  const dim3 grid1(ceil_div(l.ffn, kWaves / KW1 * 16 * FT1), l.experts), grid2(ceil_div(l.hidden, kWaves / KW2 * 16 * FT2), l.experts);
+  const dim3 small1(ceil_div(l.ffn, 16), l.experts), small2(ceil_div(l.hidden, 16), l.experts);
+  if (l.hidden >= kShort) hipLaunchKernelGGL((fc1_kernel<W, E, MT, FT1, U1, KW1, false>), grid1, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((fc1_kernel<W, E, 1, 1, 1, 4, true>), small1, dim3(256), 0, stream, a);
   NVTE_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL((fc2_kernel<W, E, MT, FT2, U2, KW2>), dim3(ceil_div(l.hidden, kWaves / KW2 * 16 * FT2), l.experts), dim3(256), 0, stream, b);
+  if (l.ffn >= kShort) hipLaunchKernelGGL((fc2_kernel<W, E, MT, FT2, U2, KW2, false>), grid2, dim3(256), 0, stream, b);
+  else hipLaunchKernelGGL((fc2_kernel<W, E, 1, 1, 1, 4, true>), small2, dim3(256), 0, stream, b);
   NVTE_CHECK_HIP(hipGetLastError());
   hipLaunchKernelGGL((combine_kernel<E>), dim3(ceil_div(l.hidden, 256), l.tokens), dim3(256), 0, stream, b.y, b.ids, out, l.top_k,
                      l.hidden, l.experts);
@@ -600,8 +614,8 @@ void nvte_amd_moe_forward(const void *x, const void *w_fc1, const void *w_fc2, c
     char *ws = static_cast<char *>(workspace);
     uint16_t *hi = reinterpret_cast<uint16_t *>(ws), *lo = reinterpret_cast<uint16_t *>(ws + hidden_bytes(l));
     float *y = reinterpret_cast<float *>(ws + 2 * hidden_bytes(l));
-    const Fc1Args a{x, w_fc1, fc1_scale_inv, topk_ids, hi, lo, l.tokens * l.top_k, l.top_k, l.hidden, l.ffn};
-    const Fc2Args b{hi, lo, w_fc2, fc2_scale_inv, topk_ids, topk_weights, y, l.tokens * l.top_k, l.hidden, l.ffn};
+    const Fc1Args a{x, w_fc1, fc1_scale_inv, topk_ids, hi, lo, l.tokens * l.top_k, l.top_k, l.experts, l.hidden, l.ffn};
+    const Fc2Args b{hi, lo, w_fc2, fc2_scale_inv, topk_ids, topk_weights, y, l.tokens * l.top_k, l.experts, l.hidden, l.ffn};
     if (wt == kNVTEFloat8E4M3) {
       t == kNVTEBFloat16 ? run<fp8_t, bf16_t>(l, a, b, out, stream) : run<fp8_t, f16_t>(l, a, b, out, stream);
     } else {
