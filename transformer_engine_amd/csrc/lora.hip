@@ -45,14 +45,14 @@ struct ShrinkArgs {
 };
 
 template <int MT, int RT, bool GUARD, bool SMALL>
-struct ShrinkBlock {  // 64 k of every row: one 128-byte line, two operands
+struct ShrinkBlock {  // 64 k of every row: one 128-byte line, 32 bytes of it per lane, two operands
   u32x4 a[MT][2], b[RT][2];
   // GUARD: the slice's ragged end, which is the row's (slices are multiples of 64)
   __device__ __forceinline__ void load(const ShrinkArgs &p, const uint16_t *const (&row)[MT], const uint16_t *const (&w)[RT], int k,
                                        int end) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = k + 32 * h, from = GUARD ? min(at, end - 8) : at;
+      const int at = k + 8 * h, from = GUARD ? min(at, end - 8) : at;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if constexpr (SMALL) a[m][h] = load8_any(row[m] + at, end - at, p.in + p.tokens * p.features);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
 #pragma unroll
   for (int m = 0; m < MT; ++m) row[m] = p.in + min(t0 + m * 16 + (lane & 15), p.tokens - 1) * p.features;
   const int begin = blockIdx.y * p.slice, end = min(begin + p.slice, p.features);
-  const int first = begin + wave * 64, kg = 8 * (lane >> 4);
+  const int first = begin + wave * 64, kg = 16 * (lane >> 4);
 
   unsigned phase = 0;
   for (uint64_t left = __ballot(id >= 0); left != 0;) {
@@ -172,11 +172,9 @@ struct ExpandArgs {
   int slices, features, rank, num, cols;  // cols: columns per workgroup, a multiple of 512
 };
 
-// A wave's step is 128 columns: operand f holds columns c0 + place(m) + f of its rows m = 0 .. 15.  D then leaves a lane (token n,
-// lane group q, register i) with the eight neighbours c0 + 32 i + 8 q + 0 .. 7 over f, so that each of the four stores of a step writes 64
-// contiguous bytes of every token.
-__device__ __forceinline__ int place(int m) { return 32 * (m & 3) + 8 * (m >> 2); }
-
+// A wave's step is 128 columns: operand f holds the columns c0 + 8 n + f, n = 0 .. 15.  D then leaves lane (n, lane group q), register i
+// with the eight neighbours c0 + 8 n + 0 .. 7 of token 4 q + i over f, so that each of the four stores of a step writes 256 contiguous
+// bytes of four tokens (tokens along the lanes instead: 64 bytes of sixteen, 119 against XX us at 8192 x 14336, rank 32).
 // Ends: a chunk of eight columns past the last takes the last eight, and its lanes write only what is theirs.  Likewise the ranks:
 // `slot_rank` says which rank operand slot s stands for (-1: none, zero in the rank vector), so that the pool is always read in whole
 // eights.  A rank past the last (RMAJOR) reads the last one again and meets such a zero.
@@ -187,7 +185,7 @@ __device__ __forceinline__ int slot_rank(int slot, int rank, bool rmajor) {
 
 template <bool RMAJOR, bool SMALL>
 __device__ __forceinline__ void pool_block(const ExpandArgs &p, int adapter, int lane, int c0, int j0, u32x4 (&f)[8]) {
-  const int c = min(c0 + place(lane & 15), max(p.features - 8, 0)), j = j0 + 8 * (lane >> 4);
+  const int c = min(c0 + 8 * (lane & 15), max(p.features - 8, 0)), j = j0 + 8 * (lane >> 4);
   const uint16_t *w = p.pool + static_cast<int64_t>(adapter) * p.rank * p.features;
   const uint16_t *end = p.pool + static_cast<int64_t>(p.num) * p.rank * p.features;
 #pragma unroll
@@ -245,14 +243,15 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
     low[n] = p.low + min(t0 + tok, p.tokens - 1) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
   }
   const int64_t stride = p.tokens * p.rank;
-  for (int s0 = 0; s0 < p.slices; s0 += 4) {
-    float part[4][kMine];
+  constexpr int kBatch = 32 / kMine;  // loads on their way at once
+  for (int s0 = 0; s0 < p.slices; s0 += kBatch) {
+    float part[kBatch][kMine];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kBatch; ++i)
 #pragma unroll
       for (int n = 0; n < kMine; ++n) part[i][n] = low[n][min(s0 + i, p.slices - 1) * stride];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kBatch; ++i)
 #pragma unroll
       for (int n = 0; n < kMine; ++n) v[n] += s0 + i < p.slices ? part[i][n] : 0.f;
   }
@@ -270,36 +269,53 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   u32x4 hi[MT][KT], lo[MT][KT];
-  int my_id[MT];
-  bool mine[MT];
+  int my_id[MT][4];       // of the lane's four tokens per subtile
+  uint32_t row[MT][4];    // their rows in the tile; one that is not written here reads the first that is
+  const int any = __builtin_ctzll(write);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    my_id[m] = __shfl(id, m * 16 + (lane & 15), 64);
-    mine[m] = (write >> (m * 16 + (lane & 15))) & 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = m * 16 + 4 * (lane >> 4) + i;
+      my_id[m][i] = __shfl(id, tok, 64);
+      row[m][i] = (((write >> tok) & 1) ? tok : any) * static_cast<uint32_t>(p.features);
+    }
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
       hi[m][k] = *reinterpret_cast<const u32x4 *>(&s_hi[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
       lo[m][k] = *reinterpret_cast<const u32x4 *>(&s_lo[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
     }
   }
-  u32x4 base[MT][4];
+  // the columns' old values travel a step ahead
+  u32x4 base[MT][4], ahead[MT][4];
+  const uint16_t *tile_base = p.base + t0 * p.features;
+  auto load_base = [&](int c0, u32x4 (&v)[MT][4]) {
+    const uint32_t c = min(c0 + 8 * (lane & 15), max(p.features - 8, 0));
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t *from = tile_base + (row[m][i] + c);
+        v[m][i] = SMALL ? load8_any(from, p.features - c, p.base + p.tokens * p.features) : load8(from);
+      }
+  };
+  if (p.base == nullptr) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) base[m][i] = ahead[m][i] = u32x4{0u, 0u, 0u, 0u};
+  } else if (c0 < end) {
+    load_base(c0, base);
+  }
   f32x4 res[MT][8];
   uint64_t left = todo;
   while (c0 < end) {
-    if (left == todo) {  // a new step: the columns' old values travel while the products run
+    if (left == todo) {  // a new step
+      if (p.base != nullptr && c0 + 512 < end) load_base(c0 + 512, ahead);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint16_t *from = p.base + min(t0 + m * 16 + (lane & 15), p.tokens - 1) * p.features;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          base[m][i] = u32x4{0u, 0u, 0u, 0u};
-          const int c = min(c0 + 32 * i + 8 * (lane >> 4), max(p.features - 8, 0));
-          if (p.base != nullptr && mine[m])
-            base[m][i] = SMALL ? load8_any(from + c, p.features - c, p.base + p.tokens * p.features) : load8(from + c);
-        }
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 8; ++i) res[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
     }
     if (left != 0) {
       const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
@@ -315,10 +331,12 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
         for (int k = 0; k < KT; ++k) {
           const Terms<E> terms(f[k][i]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m] = mfma16_split<E>(terms, hi[m][k], lo[m][k], acc[m]);
+          for (int m = 0; m < MT; ++m) acc[m] = mfma16_split<E, true>(terms, hi[m][k], lo[m][k], acc[m]);
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) res[m][i] = my_id[m] == cur ? acc[m] : res[m][i];
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) res[m][i][t] = my_id[m][t] == cur ? acc[m][t] : res[m][i][t];
       }
     }
     const bool done = left == 0;
@@ -326,13 +344,13 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
     if (done) left = todo;
     if (left != 0 && next < end) load_pool(left, next);
     if (done) {
+      const int c = c0 + 8 * (lane & 15), first = min(c, max(p.features - 8, 0));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (!mine[m]) continue;
-        uint16_t *to = p.out + (t0 + m * 16 + (lane & 15)) * p.features;
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int c = c0 + 32 * i + 8 * (lane >> 4), first = min(c, max(p.features - 8, 0));
+          if (!((write >> (m * 16 + 4 * (lane >> 4) + i)) & 1)) continue;
+          uint16_t *to = p.out + t0 * p.features + row[m][i];
           E o[8];
           const E *old = reinterpret_cast<const E *>(&base[m][i]);
 #pragma unroll
@@ -347,7 +365,10 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
               to[first + k] = static_cast<uint16_t>((k < 4 ? half[0] : half[1]) >> (16 * (k & 3)));
           }
         }
-      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) base[m][i] = ahead[m][i];
     }
     c0 = next;
   }
@@ -355,7 +376,7 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
 
 // grid: token tiles x column ranges x phases
 template <typename E, int KT, int MT, bool SMALL>
-__global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p) {
+__global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_kernel(ExpandArgs p) {
   // 16-byte aligned rows, neighbouring rows in different banks
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
   expand_tile<E, KT, MT, false, SMALL>(p, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, s_hi, s_lo);
@@ -520,7 +541,7 @@ __device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &si
 
 // the backward pass's `expand` and `pack` read the same rank vectors and nothing of each other: one launch
 template <typename E, int KT, int MT, bool SMALL>
-__global__ __launch_bounds__(256) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int phases,
+__global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int phases,
                                                           int blocks) {
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
   const int b = blockIdx.x;
@@ -565,7 +586,7 @@ struct WgradBlock {  // 32 tokens x 128 columns, and their rank vectors (zero fo
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint16_t *at = side.z + static_cast<int64_t>(tokens.t[i] & INT_MAX) * side.features + c;
-      z[i] = SMALL ? load8_any(at, side.features - c, side.z + all * side.features) : load8(at);
+      z[i] = SMALL ? load8_any(at, side.features - c, side.z + all * side.features) : load8_once(at);
     }
     const uint16_t *from = side.packed + (static_cast<int64_t>(block) * rank_tiles + j0) * 1024 + lane * 8;
 #pragma unroll
@@ -642,27 +663,42 @@ __global__ __launch_bounds__(256, RT <= 2 ? 2 : 1) void wgrad_kernel(WgradArgs p
 }
 
 // join: the sum of an adapter's work items in their order; zero for an adapter without tokens.  A workgroup takes 64 columns of
-// all ranks: dA is written as it is read, dB turned round in LDS.  grid: column pieces of both sides x adapters
+// 16 ranks: dA is written as it is read, dB turned round in LDS.  grid: column pieces of both sides x adapters x rank groups
 __global__ __launch_bounds__(256) void join_kernel(WgradArgs p, int pieces) {
-  __shared__ float s[64 * (kMaxRank + 1)];
-  const int a = blockIdx.y;
+  __shared__ float s[64][17];
+  const int a = blockIdx.y, j0 = blockIdx.z * 16;
   const bool second = static_cast<int>(blockIdx.x) >= pieces;
   const WgradSide side = second ? p.side[1] : p.side[0];
-  const int c0 = (blockIdx.x - (second ? pieces : 0)) * 64, columns = min(64, side.features - c0);
+  const int c0 = (blockIdx.x - (second ? pieces : 0)) * 64, columns = min(64, side.features - c0), ranks = min(16, p.rank - j0);
   const int first = p.plan.item_base[a], items = p.plan.item_base[a + 1] - first;
   const int64_t size = static_cast<int64_t>(p.rank) * side.features;
-  const int lane = threadIdx.x & 63;
-  for (int j = threadIdx.x >> 6; j < p.rank; j += 4) {
-    if (lane >= columns) continue;
-    const int64_t at = static_cast<int64_t>(j) * side.features + c0 + lane;
-    const float v = items > 0 ? sum_slices(side.part + first * size + at, items, size) : 0.f;
-    if (second) s[lane * (p.rank + 1) + j] = v;
-    else store1(side.grad, a * size + at, p.grad_type, v);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float *part = side.part + first * size + min(c0 + lane, side.features - 1);
+  float v[4] = {};
+  for (int i0 = 0; i0 < items; i0 += 4) {
+    float w[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        w[i][n] = part[min(i0 + i, items - 1) * size + static_cast<int64_t>(min(j0 + 4 * wave + n, p.rank - 1)) * side.features];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] += i0 + i < items ? w[i][n] : 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int j = 4 * wave + n;
+    if (second) s[lane][j] = v[n];
+    else if (lane < columns && j < ranks)
+      store1(side.grad, a * size + static_cast<int64_t>(j0 + j) * side.features + c0 + lane, p.grad_type, v[n]);
   }
   if (!second) return;
   __syncthreads();
-  for (int e = threadIdx.x; e < columns * p.rank; e += 256)
-    store1(side.grad, a * size + static_cast<int64_t>(c0) * p.rank + e, p.grad_type, s[e / p.rank * (p.rank + 1) + e % p.rank]);
+  for (int e = threadIdx.x; e < columns * 16; e += 256)
+    if ((e & 15) < ranks)
+      store1(side.grad, a * size + static_cast<int64_t>(c0 + (e >> 4)) * p.rank + j0 + (e & 15), p.grad_type, s[e >> 4][e & 15]);
 }
 
 // ====================================================================================
@@ -686,12 +722,12 @@ Shape shape_of(size_t tokens, size_t in, size_t out, size_t rank, size_t num, in
   return {static_cast<int64_t>(tokens), static_cast<int>(in), static_cast<int>(out), static_cast<int>(rank), static_cast<int>(num), t};
 }
 
-// Few tokens leave most CUs without a tile, so the features are cut into slices (a multiple of 64, at least 256) until about
-// 1024 workgroups run; whoever reads the rank vectors adds the slices.
+// Few tokens leave most CUs without a tile, so the features are cut into slices (a multiple of 64, at least 512) until about
+// 768 workgroups run, three per CU; whoever reads the rank vectors adds the slices.
 bool many_tokens(int64_t tokens) { return tokens >= 4096; }
 int slice_of(int64_t tokens, int features) {
   const int64_t tiles = std::max<int64_t>(1, ceil_div(tokens, many_tokens(tokens) ? 32 : 16));
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(1024 / tiles, ceil_div(features, 256)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(768 / tiles, ceil_div(features, 512)));
   return static_cast<int>(round_up(ceil_div(features, static_cast<size_t>(want)), 64));
 }
 int num_slices(int64_t tokens, int features) { return static_cast<int>(ceil_div(features, slice_of(tokens, features))); }
@@ -699,7 +735,7 @@ int num_slices(int64_t tokens, int features) { return static_cast<int>(ceil_div(
 // a decode tile's adapters go to workgroups of their own while there are too few of them
 int phases_of(int64_t workgroups, int64_t tokens, int num) {
   const int64_t most = std::min<int64_t>(std::min<int64_t>(num, tokens), 16);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 2048 / workgroups)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 768 / workgroups)));
 }
 
 template <typename E, int RT, int MT, int NW, int U, bool SMALL = false>
@@ -720,9 +756,9 @@ void shrink(const void *in, const void *pool, const int *ids, float *out, int64_
   if (features < 8) {
     launch_shrink<E, 8, 1, 4, 1, true>(p, slices, stream);
   } else if (rank <= 16) {
-    many ? launch_shrink<E, 1, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 1, 1, 4, 2>(p, slices, stream);
+    many ? launch_shrink<E, 1, 2, 4, 1>(p, slices, stream) : launch_shrink<E, 1, 1, 4, 2>(p, slices, stream);
   } else if (rank <= 32) {
-    many ? launch_shrink<E, 2, 2, 4, 2>(p, slices, stream) : launch_shrink<E, 2, 1, 4, 2>(p, slices, stream);
+    many ? launch_shrink<E, 2, 2, 4, 1>(p, slices, stream) : launch_shrink<E, 2, 1, 4, 2>(p, slices, stream);
   } else if (rank <= 64) {
     many ? launch_shrink<E, 4, 2, 4, 1>(p, slices, stream) : launch_shrink<E, 4, 1, 4, 1>(p, slices, stream);
   } else {
@@ -744,9 +780,9 @@ void expand_variant(int rank, int64_t tokens, bool small_features, bool small_ra
   else launch(Four(), One(), std::false_type());
 }
 
-// columns per workgroup: 512 until there are about 2048 workgroups
+// columns per workgroup: 512 until there are about 1024 workgroups
 int columns_of(int64_t tiles, int features) {
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(features, 512), 2048 / tiles));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(features, 512), 1024 / tiles));
   return static_cast<int>(round_up(ceil_div(features, static_cast<size_t>(want)), 512));
 }
 
@@ -865,7 +901,7 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   NVTE_CHECK(items <= 65535, "too many work items: ", items);
   if (items > 0) launch_wgrad<E>(p, static_cast<unsigned>(items), stream);
   const int columns = static_cast<int>(ceil_div(s.in, 64));
-  hipLaunchKernelGGL(join_kernel, dim3(columns + ceil_div(s.out, 64), s.num), dim3(256), 0, stream, p, columns);
+  hipLaunchKernelGGL(join_kernel, dim3(columns + ceil_div(s.out, 64), s.num, ceil_div(s.rank, 16)), dim3(256), 0, stream, p, columns);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 

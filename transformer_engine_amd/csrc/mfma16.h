@@ -88,6 +88,10 @@ __device__ __forceinline__ f32x4 mfma16_split(const Terms<E> &w, u32x4 hi, u32x4
 // lengths nor shifted storage need kernels of their own.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ u32x4 load8(const uint16_t *p) { return *reinterpret_cast<const u32x4_any *>(p); }
+// for what is read once per call: does not displace what other workgroups share in L2
+__device__ __forceinline__ u32x4 load8_once(const uint16_t *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+}
 __device__ __forceinline__ void store8(uint16_t *p, u32x4 v) { *reinterpret_cast<u32x4_any *>(p) = v; }
 // The ends of rows whose length is no multiple of the step: a lane whose eight elements would reach past the end takes the last
 // eight instead and, where they are summed, has the `skip` that its neighbour holds already set to zero.  This keeps the kernels

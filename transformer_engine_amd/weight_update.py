@@ -14,6 +14,9 @@ not provided.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from contextlib import nullcontext
+from operator import attrgetter
 from typing import List, Optional, Sequence
 
 import torch
@@ -125,28 +128,40 @@ multi_tensor_applier = MultiTensorApply(2048 * 32)
 # =====================================================================================
 # global gradient norm and clipping
 # =====================================================================================
+_dtype_of = attrgetter("dtype")
 _GRAD_DTYPES = {torch.float32: int(DType.kFloat32), torch.float16: int(DType.kFloat16), torch.bfloat16: int(DType.kBFloat16)}
 
 
 class _Arrays:
-    """Host arrays of addresses, element counts and dtypes for the list entry points of amd_ext.h."""
+    """Host arrays of addresses, element counts and dtypes for the list entry points of amd_ext.h.  Lists of hundreds of small
+    gradients are bound by this, so every question is put to all tensors at once."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], name: str):
         n = len(tensors)
-        self.n, self.device = n, tensors[0].device if n else torch.device("cuda", torch.cuda.current_device())
+        devices = set(map(torch.Tensor.get_device, tensors))
+        dtypes = set(map(_dtype_of, tensors))
+        if not (len(devices) <= 1 and -1 not in devices and dtypes <= _GRAD_DTYPES.keys()
+                and all(map(torch.Tensor.is_contiguous, tensors))):
+            self._complain(tensors, name)
+        self.n, self.device = n, devices.pop() if n else torch.cuda.current_device()
+        self.ptrs = array("Q", map(torch.Tensor.data_ptr, tensors))
+        self.numels = array("Q", map(torch.Tensor.numel, tensors))
+        self.dtypes = (array("i", [_GRAD_DTYPES[dtypes.pop()]]) * n if len(dtypes) == 1
+                       else array("i", map(_GRAD_DTYPES.__getitem__, map(_dtype_of, tensors))))
+        self.ptrs_at, self.numels_at, self.dtypes_at = (a.buffer_info()[0] for a in (self.ptrs, self.numels, self.dtypes))
+
+    @staticmethod
+    def _complain(tensors, name):
         for i, t in enumerate(tensors):
             if not t.is_cuda:
                 raise RuntimeError(f"{name}[{i}] is on {t.device}: gradients are clipped on the GPU only (no CPU fallback in this "
                                    "library)")
-            if t.device != self.device:
-                raise ValueError(f"{name}[{i}] is on {t.device}, but {name}[0] is on {self.device}")
+            if t.device != tensors[0].device:
+                raise ValueError(f"{name}[{i}] is on {t.device}, but {name}[0] is on {tensors[0].device}")
             if t.dtype not in _GRAD_DTYPES:
                 raise TypeError(f"{name}[{i}] must be float32, float16 or bfloat16, got {t.dtype}")
             if not t.is_contiguous():
                 raise ValueError(f"{name}[{i}] must be contiguous")
-        self.ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in tensors])
-        self.numels = (C.c_size_t * n)(*[t.numel() for t in tensors])
-        self.dtypes = (C.c_int * n)(*[_GRAD_DTYPES[t.dtype] for t in tensors])
 
 
 def _all_reduce_sum(t: torch.Tensor, group):
@@ -169,17 +184,21 @@ def grad_norm(grads: Sequence[torch.Tensor], group=None) -> torch.Tensor:
 
 def _grad_norm(grads, group):
     arr = _Arrays(grads, "grads")
-    with torch.cuda.device(arr.device):
-        norm = torch.empty(1, dtype=torch.float32, device=arr.device)
-        total = torch.empty(1, dtype=torch.float64, device=arr.device)
-        size = api.nvte_amd_grad_norm_workspace_size(arr.numels, arr.n)
-        ws = torch.empty(size, dtype=torch.uint8, device=arr.device)
-        api.nvte_amd_grad_norm(arr.ptrs, arr.numels, arr.dtypes, arr.n, total.data_ptr(), norm.data_ptr(), ws.data_ptr(), size,
-                               current_stream_ptr())
+    with _on(arr.device):
+        norm = torch.empty(1, dtype=torch.float32, device="cuda")
+        total = torch.empty(1, dtype=torch.float64, device="cuda")
+        size = api.nvte_amd_grad_norm_workspace_size(arr.numels_at, arr.n)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        api.nvte_amd_grad_norm(arr.ptrs_at, arr.numels_at, arr.dtypes_at, arr.n, total.data_ptr(), norm.data_ptr(), ws.data_ptr(),
+                               size, current_stream_ptr())
         if group is not None:
             _all_reduce_sum(total, group)
             norm = total.sqrt().to(torch.float32)
     return total, norm, arr
+
+
+def _on(device: int):
+    return nullcontext() if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, outs: Optional[Sequence[torch.Tensor]] = None,
@@ -194,26 +213,27 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, outs: Optiona
     outs = grads if outs is None else list(outs)
     if len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients, but {len(outs)} outputs")
-    for i, (g, o) in enumerate(zip(grads, outs)):
-        if g is not o and g.numel() != o.numel():
-            raise ValueError(f"grads[{i}] has {g.numel()} elements, but outs[{i}] has {o.numel()}")
     if group is not None:
         total, norm, arr = _grad_norm(grads, group)
     else:
         arr = _Arrays(grads, "grads")
     out = arr if outs is grads else _Arrays(outs, "outs")
     if arr.device != out.device:
-        raise ValueError(f"grads are on {arr.device}, but outs are on {out.device}")
-    with torch.cuda.device(arr.device):
+        raise ValueError(f"grads are on cuda:{arr.device}, but outs are on cuda:{out.device}")
+    if arr.numels != out.numels:
+        i = next(i for i in range(arr.n) if arr.numels[i] != out.numels[i])
+        raise ValueError(f"grads[{i}] has {arr.numels[i]} elements, but outs[{i}] has {out.numels[i]}")
+    with _on(arr.device):
         if group is not None:
-            api.nvte_amd_clip_by_sum_of_squares(arr.ptrs, out.ptrs, arr.numels, arr.dtypes, out.dtypes, arr.n, total.data_ptr(),
-                                                C.c_float(max_norm), C.c_float(eps), norm.data_ptr(), current_stream_ptr())
+            api.nvte_amd_clip_by_sum_of_squares(arr.ptrs_at, out.ptrs_at, arr.numels_at, arr.dtypes_at, out.dtypes_at, arr.n,
+                                                total.data_ptr(), C.c_float(max_norm), C.c_float(eps), norm.data_ptr(),
+                                                current_stream_ptr())
             return norm
-        norm = torch.empty(1, dtype=torch.float32, device=arr.device)
-        size = api.nvte_amd_grad_norm_workspace_size(arr.numels, arr.n)
-        ws = torch.empty(size, dtype=torch.uint8, device=arr.device)
-        api.nvte_amd_clip_grad_norm(arr.ptrs, out.ptrs, arr.numels, arr.dtypes, out.dtypes, arr.n, C.c_float(max_norm),
-                                    C.c_float(eps), norm.data_ptr(), ws.data_ptr(), size, current_stream_ptr())
+        norm = torch.empty(1, dtype=torch.float32, device="cuda")
+        size = api.nvte_amd_grad_norm_workspace_size(arr.numels_at, arr.n)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        api.nvte_amd_clip_grad_norm(arr.ptrs_at, out.ptrs_at, arr.numels_at, arr.dtypes_at, out.dtypes_at, arr.n,
+                                    C.c_float(max_norm), C.c_float(eps), norm.data_ptr(), ws.data_ptr(), size, current_stream_ptr())
     return norm
 
 
