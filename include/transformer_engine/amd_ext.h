@@ -107,15 +107,17 @@ void nvte_amd_clip_by_sum_of_squares(const void *const *grads, void *const *outs
 
 /* ---- Low-rank adapters of many requests beside a shared projection (Python: lora.py).
  * x [tokens, in], a [num_adapters, rank, in], b [num_adapters, out, rank], base / out [tokens, out], all of one dtype (bf16 or
- * fp16), contiguous; adapter_ids [tokens] int32, any order, a value outside [0, num_adapters) = no adapter; scaling
+ * fp16), contiguous; up to 2^27 tokens; adapter_ids [tokens] int32, any order, a value outside [0, num_adapters) = no adapter; scaling
  * [num_adapters] fp32 or NULL (1); base NULL = zero, or out itself.  rank 1 to 128, any feature sizes.
  *   low[t] = a[id] x[t]        out[t] = base[t] + scaling[id] b[id] low[t]
  * low [nvte_amd_lora_num_slices(tokens, in), tokens, rank] fp32: partial sums of the rank vectors, which the backward pass reads
  * (rows without an adapter are not written).  A non-finite weight or activation makes its own rows non-finite and no other. */
 size_t nvte_amd_lora_num_slices(size_t tokens, size_t features);
+size_t nvte_amd_lora_forward_workspace_size(size_t tokens, size_t num_adapters);   /* 0: workspace may be NULL */
 void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const int *adapter_ids, const float *scaling,
                            const void *base, void *out, float *low, size_t tokens, size_t in_features, size_t out_features,
-                           size_t rank, size_t num_adapters, int dtype, hipStream_t stream);
+                           size_t rank, size_t num_adapters, int dtype, void *workspace, size_t workspace_bytes,
+                           hipStream_t stream);
 /* dx[t] = base_grad[t] + scaling[id] a[id]^T (b[id]^T dy[t]); da [num_adapters, rank, in] and db [num_adapters, out, rank], in
  * dtype or fp32 (grad_dtype), are sums over each adapter's tokens in a fixed order, zero for an adapter without tokens.  dx may
  * be NULL, da and db may be NULL together; base_grad NULL = zero, or dx itself.  Up to 4096 adapters when da / db are wanted. */

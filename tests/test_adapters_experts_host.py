@@ -11,7 +11,8 @@ P = 0x1000
 
 
 def lora_forward(**k):
-    d = dict(x=P, a=P, b=P, ids=P, scaling=0, base=0, out=P, low=P, tokens=4, k=16, o=16, r=8, n=2, dtype=kBFloat16)
+    d = dict(x=P, a=P, b=P, ids=P, scaling=0, base=0, out=P, low=P, tokens=4, k=16, o=16, r=8, n=2, dtype=kBFloat16,
+             ws=P, size=1 << 20)
     d.update(k)
     api.nvte_amd_lora_forward(*d.values(), 0)
 
@@ -42,6 +43,13 @@ def test_lora_backward_refusals(bad):
 def test_lora_forward_refuses_no_output():
     with pytest.raises(NVTEError):
         lora_forward(out=0)
+
+
+@pytest.mark.parametrize("bad", [dict(ws=0), dict(size=64), dict(ws=P + 8)])
+def test_lora_forward_refuses_a_bad_workspace(bad):
+    assert api.nvte_amd_lora_forward_workspace_size(4, 2) == 0 < api.nvte_amd_lora_forward_workspace_size(2000, 2)
+    with pytest.raises(NVTEError, match="workspace"):
+        lora_forward(tokens=2000, **bad)
 
 
 def test_lora_sizes():

@@ -121,7 +121,8 @@ _SIGS = {
     "nvte_amd_clip_grad_norm": (_V, [_P, _P, _P, _P, _P, _SZ, _F, _F, _P, _P, _SZ, _P]),
     "nvte_amd_clip_by_sum_of_squares": (_V, [_P, _P, _P, _P, _P, _SZ, _P, _F, _F, _P, _P]),
     "nvte_amd_lora_num_slices": (_SZ, [_SZ, _SZ]),
-    "nvte_amd_lora_forward": (_V, [_P] * 8 + [_SZ] * 5 + [_I, _P]),
+    "nvte_amd_lora_forward_workspace_size": (_SZ, [_SZ, _SZ]),
+    "nvte_amd_lora_forward": (_V, [_P] * 8 + [_SZ] * 5 + [_I, _P, _SZ, _P]),
     "nvte_amd_lora_backward_workspace_size": (_SZ, [_SZ] * 5),
     "nvte_amd_lora_backward": (_V, [_P] * 11 + [_SZ] * 5 + [_I, _I, _P, _SZ, _P]),
     "nvte_amd_moe_topk": (_V, [_P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _P]),

@@ -25,6 +25,7 @@ namespace te {
 namespace {
 
 constexpr int kMaxRank = 128;
+constexpr size_t kMaxTokens = 1u << 27;  // keeps every grid below 2^32 threads
 constexpr int kMaxAdapters = 4096;  // of a backward pass: the plan kernel's histogram in LDS
 
 __device__ __forceinline__ int valid_id(const int *ids, int64_t t, int64_t tokens, int num) {
@@ -33,12 +34,50 @@ __device__ __forceinline__ int valid_id(const int *ids, int64_t t, int64_t token
   return id >= 0 && id < num ? id : -1;
 }
 
+constexpr int kBlock = 32;
+
+// The tokens of every adapter in rising order, then those without one; each list padded to whole blocks with its last token, marked
+// by the sign bit (see `prepare`).
+struct Plan {
+  const int *order;       // [most_blocks * 32]; null: tokens are taken as they come
+  const int *block_base;  // [num + 2] first block of every adapter in `order`, of the rest, and the end
+  const int *item_base;   // [num + 1] first work item of every adapter
+};
+
+// the adapter whose range of `base` holds `i` (one without tokens holds none)
+__device__ __forceinline__ int owner_of(const int *base, int num, int i) {
+  int a = 0;
+  for (int hi = num; hi - a > 1;) {
+    const int mid = (a + hi) >> 1;
+    if (base[mid] <= i) a = mid; else hi = mid;
+  }
+  return a;
+}
+
+// a lane's token of a tile of 16 MT, and its adapter: -1 none, -2 no token
+struct TileToken {
+  int64_t t;
+  int id;
+};
+__device__ __forceinline__ TileToken tile_token(const Plan &plan, const int *ids, int64_t tile, int size, int lane, int64_t tokens,
+                                                int num) {
+  if (plan.order == nullptr) {
+    const int64_t t = tile * size + lane;
+    return {min(t, tokens - 1), lane < size && t < tokens ? valid_id(ids, t, tokens, num) : -2};
+  }
+  const int block = static_cast<int>(tile * size / kBlock);
+  if (block >= plan.block_base[num + 1]) return {0, -2};
+  const int v = plan.order[tile * size + min(lane, size - 1)], a = owner_of(plan.block_base, num + 1, block);
+  return {v & INT_MAX, lane < size && v >= 0 ? (a < num ? a : -1) : -2};
+}
+
 // ====================================================================================
 // shrink: out[slice][t][j] = sum over the slice's k of in[t][k] * pool[a][j][k]
 // ====================================================================================
 struct ShrinkArgs {
   const uint16_t *in, *pool;
   const int *ids;
+  Plan plan;
   float *out;
   int64_t tokens;
   int features, rank, num, slice;
@@ -84,11 +123,11 @@ template <typename E, int RT, int MT, int NW, int U, bool SMALL>
 __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
   __shared__ f32x4 red[NW][MT * RT][64];
   const int lane = threadIdx.x & 63, wave = wave_index();
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * MT);
-  const int id = lane < 16 * MT ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
+  const TileToken own = tile_token(p.plan, p.ids, blockIdx.x, 16 * MT, lane, p.tokens, p.num);
+  const int id = own.id, token = static_cast<int>(own.t);
   const uint16_t *row[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) row[m] = p.in + min(t0 + m * 16 + (lane & 15), p.tokens - 1) * p.features;
+  for (int m = 0; m < MT; ++m) row[m] = p.in + static_cast<int64_t>(__shfl(token, m * 16 + (lane & 15), 64)) * p.features;
   const int begin = blockIdx.y * p.slice, end = min(begin + p.slice, p.features);
   const int first = begin + wave * 64, kg = 16 * (lane >> 4);
 
@@ -139,7 +178,8 @@ __global__ __launch_bounds__(NW * 64) void shrink_kernel(ShrinkArgs p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int tok = m * 16 + (l >> 4) * 4 + i;
-        if (((mine >> tok) & 1) && col < p.rank) p.out[(blockIdx.y * p.tokens + t0 + tok) * p.rank + col] = s[i];
+        const int64_t t = __shfl(token, tok, 64);
+        if (((mine >> tok) & 1) && col < p.rank) p.out[(blockIdx.y * p.tokens + t) * p.rank + col] = s[i];
       }
     }
   }
@@ -167,6 +207,7 @@ struct ExpandArgs {
   const uint16_t *pool, *base;  // base may be null (zero) or out itself
   const float *scaling;         // null: 1
   const int *ids;
+  Plan plan;
   uint16_t *out;
   int64_t tokens;
   int slices, features, rank, num, cols;  // cols: columns per workgroup, a multiple of 512
@@ -205,10 +246,9 @@ template <typename E, int KT, int MT, bool RMAJOR, bool SMALL>
 __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, int columns, unsigned my_phase, unsigned phases,
                                             uint16_t (*s_hi)[KT * 32 + 8], uint16_t (*s_lo)[KT * 32 + 8]) {
   const int lane = threadIdx.x & 63, wave = wave_index();
-  const int64_t t0 = tile * (16 * MT);
-  const int id = lane < 16 * MT ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
-  const bool without = lane < 16 * MT && t0 + lane < p.tokens && id < 0;
-  uint64_t todo = __ballot(id >= 0), write = my_phase == 0 && p.base != p.out ? __ballot(without) : 0;
+  const TileToken own = tile_token(p.plan, p.ids, tile, 16 * MT, lane, p.tokens, p.num);
+  const int id = own.id, token = static_cast<int>(own.t);
+  uint64_t todo = __ballot(id >= 0), write = my_phase == 0 && p.base != p.out ? __ballot(id == -1) : 0;
   if (phases > 1) {
     unsigned phase = 0;
     uint64_t left = todo;
@@ -240,7 +280,7 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
 #pragma unroll
   for (int n = 0; n < kMine; ++n) {
     const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
-    low[n] = p.low + min(t0 + tok, p.tokens - 1) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
+    low[n] = p.low + static_cast<int64_t>(__shfl(token, tok, 64)) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
   }
   const int64_t stride = p.tokens * p.rank;
   constexpr int kBatch = 32 / kMine;  // loads on their way at once
@@ -270,7 +310,7 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   asm volatile("" ::: "memory");
   u32x4 hi[MT][KT], lo[MT][KT];
   int my_id[MT][4];       // of the lane's four tokens per subtile
-  uint32_t row[MT][4];    // their rows in the tile; one that is not written here reads the first that is
+  int row[MT][4];         // they themselves; one that is not written here reads the first that is
   const int any = __builtin_ctzll(write);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -278,7 +318,7 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
     for (int i = 0; i < 4; ++i) {
       const int tok = m * 16 + 4 * (lane >> 4) + i;
       my_id[m][i] = __shfl(id, tok, 64);
-      row[m][i] = (((write >> tok) & 1) ? tok : any) * static_cast<uint32_t>(p.features);
+      row[m][i] = __shfl(token, ((write >> tok) & 1) ? tok : any, 64);
     }
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
@@ -288,14 +328,13 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   }
   // the columns' old values travel a step ahead
   u32x4 base[MT][4], ahead[MT][4];
-  const uint16_t *tile_base = p.base + t0 * p.features;
   auto load_base = [&](int c0, u32x4 (&v)[MT][4]) {
-    const uint32_t c = min(c0 + 8 * (lane & 15), max(p.features - 8, 0));
+    const int c = min(c0 + 8 * (lane & 15), max(p.features - 8, 0));
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint16_t *from = tile_base + (row[m][i] + c);
+        const uint16_t *from = p.base + (static_cast<int64_t>(row[m][i]) * p.features + c);
         v[m][i] = SMALL ? load8_any(from, p.features - c, p.base + p.tokens * p.features) : load8(from);
       }
   };
@@ -350,7 +389,7 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (!((write >> (m * 16 + 4 * (lane >> 4) + i)) & 1)) continue;
-          uint16_t *to = p.out + t0 * p.features + row[m][i];
+          uint16_t *to = p.out + static_cast<int64_t>(row[m][i]) * p.features;
           E o[8];
           const E *old = reinterpret_cast<const E *>(&base[m][i]);
 #pragma unroll
@@ -383,25 +422,18 @@ __global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_kernel(ExpandArgs
 }
 
 // ====================================================================================
-// prepare: the tokens of every adapter in rising order, each adapter's list padded to whole blocks of 32 with its last token, marked
-// by the sign bit; where they begin; where its work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to [rank][features].
+// prepare: the lists of a Plan, and where each adapter's work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to
+// [rank][features].
 // One workgroup per adapter counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged; its sixteen waves own
 // consecutive stretches of the tokens.
 // ====================================================================================
-constexpr int kBlock = 32;
-
-struct Plan {
-  int *order;       // [most_blocks * 32]
-  int *block_base;  // [num + 1] first block of every adapter in `order`
-  int *item_base;   // [num + 1] first work item of every adapter
-};
 struct PrepareArgs {
   const int *ids;
-  const uint16_t *pool;  // null: no transpose
+  const uint16_t *pool;
   uint16_t *transposed;
-  Plan plan;             // order null: no lists
+  int *order, *block_base, *item_base;
   int64_t tokens;
-  int features, rank, num, per_item, lists;  // lists: workgroups of the first part
+  int features, rank, num, per_item, lists;  // lists: workgroups of the first part, num + 1 or none
 };
 
 __device__ __forceinline__ int sum_1024(int v, int *scratch) {  // valid in every thread
@@ -416,14 +448,21 @@ __device__ __forceinline__ int sum_1024(int v, int *scratch) {  // valid in ever
   return s;
 }
 
+// a == num: the tokens without an adapter
 __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t stretch = ((p.tokens + 15) / 16 + 63) / 64 * 64, from = wave * stretch;
   const int64_t to = min(from + stretch, p.tokens);
-  for (int i = threadIdx.x; i < p.num; i += 1024) hist[i] = 0;
+  // its adapter, num for none; -1 past the stretch
+  auto id_of = [&](int64_t t) {
+    if (t >= to) return -1;
+    const int id = p.ids[t];
+    return id >= 0 && id < p.num ? id : p.num;
+  };
+  for (int i = threadIdx.x; i <= p.num; i += 1024) hist[i] = 0;
   __syncthreads();
   for (int64_t t0 = from; t0 < to; t0 += 64) {
-    const int id = t0 + lane < to ? valid_id(p.ids, t0 + lane, p.tokens, p.num) : -1;
+    const int id = id_of(t0 + lane);
     for (uint64_t left = __ballot(id >= 0); left != 0;) {  // one addition per distinct id: a run would queue up on one address
       const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
       const uint64_t same = __ballot(id == cur);
@@ -442,29 +481,25 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   items = sum_1024(items, scratch);
   const int mine = hist[a], my_blocks = (mine + kBlock - 1) / kBlock;
   if (threadIdx.x == 0) {
-    p.plan.block_base[a] = blocks;
-    p.plan.item_base[a] = items;
-    if (a == p.num - 1) {
-      p.plan.block_base[p.num] = blocks + my_blocks;
-      p.plan.item_base[p.num] = items + (my_blocks + p.per_item - 1) / p.per_item;
-    }
+    p.block_base[a] = blocks;
+    p.item_base[a] = items;  // that of a == num is the end
+    if (a == p.num) p.block_base[a + 1] = blocks + my_blocks;
   }
   if (mine == 0) return;
-  int *order = p.plan.order + static_cast<int64_t>(blocks) * kBlock;
+  int *order = p.order + static_cast<int64_t>(blocks) * kBlock;
   int count = 0;
-  for (int64_t t0 = from; t0 < to; t0 += 64)
-    count += __popcll(__ballot(t0 + lane < to && p.ids[t0 + lane] == a));
+  for (int64_t t0 = from; t0 < to; t0 += 64) count += __popcll(__ballot(id_of(t0 + lane) == a));
   __syncthreads();
   if (lane == 0) scratch[wave] = count;
   __syncthreads();
   int at = 0;
   for (int w = 0; w < wave; ++w) at += scratch[w];
   for (int64_t t0 = from; t0 < to; t0 += 64) {
-    const bool hit = t0 + lane < to && p.ids[t0 + lane] == a;
+    const bool hit = id_of(t0 + lane) == a;
     const uint64_t m = __ballot(hit);
-    const int to_slot = at + __popcll(m & ((1ull << lane) - 1)), t = static_cast<int>(t0) + lane;
-    if (hit) order[to_slot] = t;
-    if (hit && to_slot == mine - 1)
+    const int slot = at + __popcll(m & ((1ull << lane) - 1)), t = static_cast<int>(t0) + lane;
+    if (hit) order[slot] = t;
+    if (hit && slot == mine - 1)
       for (int i = mine; i < my_blocks * kBlock; ++i) order[i] = t | INT_MIN;
     at += __popcll(m);
   }
@@ -487,7 +522,7 @@ __device__ void transpose_rows(const PrepareArgs &p, int64_t piece, uint16_t *s)
 
 __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
   __shared__ union {
-    int hist[kMaxAdapters];
+    int hist[kMaxAdapters + 1];
     uint16_t rows[64 * (kMaxRank + 1)];
   } s;
   __shared__ int scratch[16];
@@ -510,16 +545,6 @@ struct PackArgs {
   int64_t tokens;
   int rank, num;
 };
-
-// the adapter whose range of `base` holds `i` (adapters without tokens have none)
-__device__ __forceinline__ int owner_of(const int *base, int num, int i) {
-  int a = 0;
-  for (int hi = num; hi - a > 1;) {
-    const int mid = (a + hi) >> 1;
-    if (base[mid] <= i) a = mid; else hi = mid;
-  }
-  return a;
-}
 
 __device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &side, int block) {
   if (block >= p.plan.block_base[p.num]) return;
@@ -718,7 +743,7 @@ Shape shape_of(size_t tokens, size_t in, size_t out, size_t rank, size_t num, in
   NVTE_CHECK(rank >= 1 && rank <= kMaxRank, "rank must be 1 to ", kMaxRank, ", got ", rank);
   NVTE_CHECK(in >= 1 && in <= (1u << 24) && out >= 1 && out <= (1u << 24), "features must be 1 to 2^24, got ", in, " and ", out);
   NVTE_CHECK(num >= 1 && num <= INT_MAX, "at least one adapter is needed, got ", num);
-  NVTE_CHECK(tokens < (1ull << 31) - 64, "too many tokens: ", tokens);
+  NVTE_CHECK(tokens <= kMaxTokens, "up to ", kMaxTokens, " tokens per call, got ", tokens);
   return {static_cast<int64_t>(tokens), static_cast<int>(in), static_cast<int>(out), static_cast<int>(rank), static_cast<int>(num), t};
 }
 
@@ -738,19 +763,29 @@ int phases_of(int64_t workgroups, int64_t tokens, int num) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 768 / workgroups)));
 }
 
+// every list's last block may be partly filled
+int64_t most_blocks(int64_t tokens, int num) { return tokens / kBlock + std::min<int64_t>(num + 1, tokens); }
+int64_t tiles_of(const Plan &plan, int64_t tokens, int num, int size) {
+  return plan.order != nullptr ? most_blocks(tokens, num) * kBlock / size : static_cast<int64_t>(ceil_div(tokens, size));
+}
+
+// Tokens are put in order of their adapters first where tiles would otherwise walk through many: a batch of 8192 with 64 adapters in any
+// order took 1356 us without and XX us with it; one whose requests lie back to back pays the extra launch (XX us at 2931 tokens).
+bool ordered(int64_t tokens, int num) { return tokens >= 1024 && num > 1 && num <= kMaxAdapters; }
+
 template <typename E, int RT, int MT, int NW, int U, bool SMALL = false>
 void launch_shrink(const ShrinkArgs &p, int slices, hipStream_t stream) {
-  const int64_t tiles = (p.tokens + 16 * MT - 1) / (16 * MT);
-  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, U, SMALL>), dim3(tiles, slices, phases_of(tiles * slices, p.tokens, p.num)),
-                     dim3(NW * 64), 0, stream, p);
+  const int64_t tiles = tiles_of(p.plan, p.tokens, p.num, 16 * MT);
+  const int phases = p.plan.order != nullptr ? 1 : phases_of(tiles * slices, p.tokens, p.num);
+  hipLaunchKernelGGL((shrink_kernel<E, RT, MT, NW, U, SMALL>), dim3(tiles, slices, phases), dim3(NW * 64), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
 template <typename E>
-void shrink(const void *in, const void *pool, const int *ids, float *out, int64_t tokens, int features, int rank, int num,
-            hipStream_t stream) {
-  const ShrinkArgs p{static_cast<const uint16_t *>(in), static_cast<const uint16_t *>(pool), ids, out, tokens, features, rank, num,
-                     slice_of(tokens, features)};
+void shrink(const void *in, const void *pool, const int *ids, const Plan &plan, float *out, int64_t tokens, int features, int rank,
+            int num, hipStream_t stream) {
+  const ShrinkArgs p{static_cast<const uint16_t *>(in), static_cast<const uint16_t *>(pool), ids, plan, out, tokens, features, rank,
+                     num, slice_of(tokens, features)};
   const int slices = num_slices(tokens, features);
   const bool many = many_tokens(tokens);
   if (features < 8) {
@@ -789,11 +824,11 @@ int columns_of(int64_t tiles, int features) {
 template <typename E>
 void expand(ExpandArgs p, hipStream_t stream) {
   expand_variant(p.rank, p.tokens, p.features < 8, p.rank < 8, [&](auto kt, auto mt, auto small) {
-    const int64_t tiles = ceil_div(p.tokens, 16 * mt());
+    const int64_t tiles = tiles_of(p.plan, p.tokens, p.num, 16 * mt());
     p.cols = columns_of(tiles, p.features);
     const int64_t ranges = ceil_div(p.features, p.cols);
-    hipLaunchKernelGGL((expand_kernel<E, kt(), mt(), small()>), dim3(tiles, ranges, phases_of(tiles * ranges, p.tokens, p.num)),
-                       dim3(256), 0, stream, p);
+    const int phases = p.plan.order != nullptr ? 1 : phases_of(tiles * ranges, p.tokens, p.num);
+    hipLaunchKernelGGL((expand_kernel<E, kt(), mt(), small()>), dim3(tiles, ranges, phases), dim3(256), 0, stream, p);
     NVTE_CHECK_HIP(hipGetLastError());
   });
 }
@@ -801,12 +836,12 @@ void expand(ExpandArgs p, hipStream_t stream) {
 template <typename E>
 void expand_and_pack(ExpandArgs p, const PackArgs &q, int64_t blocks, hipStream_t stream) {
   expand_variant(p.rank, p.tokens, p.features < 8, false, [&](auto kt, auto mt, auto small) {
-    const int64_t tiles = ceil_div(p.tokens, 16 * mt());
+    const int64_t tiles = tiles_of(p.plan, p.tokens, p.num, 16 * mt());
     p.cols = columns_of(tiles, p.features);
     const int64_t ranges = p.out != nullptr ? ceil_div(p.features, p.cols) : 0;
-    const int phases = phases_of(std::max<int64_t>(1, tiles * ranges), p.tokens, p.num);
+    const int phases = p.plan.order != nullptr ? 1 : phases_of(std::max<int64_t>(1, tiles * ranges), p.tokens, p.num);
     const int64_t grid = 2 * blocks + tiles * ranges * phases;
-    NVTE_CHECK(grid <= INT_MAX, "too many workgroups: ", grid);
+    NVTE_CHECK(grid < (1 << 24), "too many workgroups: ", grid);
     if (grid == 0) return;
     hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt(), small()>), dim3(grid), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
                        static_cast<int>(tiles), phases, static_cast<int>(blocks));
@@ -830,9 +865,33 @@ int blocks_per_item(const Shape &s) {
   const int64_t items = std::max<int64_t>(1, 512 / columns);
   return static_cast<int>(std::max<size_t>(2, ceil_div(ceil_div(s.tokens, kBlock), items)));
 }
-// every adapter's last block (item) may be partly filled
-int64_t most_blocks(const Shape &s) { return s.tokens / kBlock + std::min<int64_t>(s.num, s.tokens); }
-int64_t most_items(const Shape &s) { return most_blocks(s) / blocks_per_item(s) + std::min<int64_t>(s.num, s.tokens); }
+int64_t most_items(const Shape &s) {
+  return most_blocks(s.tokens, s.num) / blocks_per_item(s) + std::min<int64_t>(s.num, s.tokens);
+}
+
+// one launch: the lists, if wanted, and B transposed, if given
+Plan prepare(const Shape &s, const int *ids, bool lists, const void *b, uint16_t *transposed, int *order, int *block_base,
+             int *item_base, hipStream_t stream) {
+  const int64_t pieces = b != nullptr ? static_cast<int64_t>(s.num) * ceil_div(s.out, 64) : 0, first = lists ? s.num + 1 : 0;
+  NVTE_CHECK(first + pieces < (1 << 22), "too many adapters to transpose: ", s.num);
+  const PrepareArgs p{ids, static_cast<const uint16_t *>(b), transposed, order, block_base, item_base, s.tokens, s.out, s.rank, s.num,
+                      blocks_per_item(s), static_cast<int>(first)};
+  hipLaunchKernelGGL(prepare_kernel, dim3(first + pieces), dim3(1024), 0, stream, p);
+  NVTE_CHECK_HIP(hipGetLastError());
+  return {order, block_base, item_base};
+}
+
+struct ForwardWorkspace {
+  size_t order, block_base, item_base, bytes;
+};
+ForwardWorkspace forward_workspace(int64_t tokens, int num) {
+  if (!ordered(tokens, num)) return {};
+  ForwardWorkspace w{};
+  w.block_base = round_up(most_blocks(tokens, num) * kBlock * sizeof(int), 256);
+  w.item_base = w.block_base + round_up((num + 2) * sizeof(int), 256);
+  w.bytes = w.item_base + round_up((num + 1) * sizeof(int), 256);
+  return w;
+}
 
 struct BackwardWorkspace {
   size_t low, transposed, order, block_base, item_base, packed_a, packed_b, part_a, part_b, bytes;
@@ -847,10 +906,10 @@ BackwardWorkspace backward_workspace(const Shape &s) {
   };
   w.low = take(static_cast<size_t>(num_slices(s.tokens, s.out)) * s.tokens * s.rank * sizeof(float));
   w.transposed = take(static_cast<size_t>(s.num) * s.rank * s.out * 2);
-  w.order = take(most_blocks(s) * kBlock * sizeof(int));
-  w.block_base = take((s.num + 1) * sizeof(int));
+  w.order = take(most_blocks(s.tokens, s.num) * kBlock * sizeof(int));
+  w.block_base = take((s.num + 2) * sizeof(int));
   w.item_base = take((s.num + 1) * sizeof(int));
-  const size_t packed = static_cast<size_t>(most_blocks(s)) * ceil_div(s.rank, 16) * 2048;
+  const size_t packed = static_cast<size_t>(most_blocks(s.tokens, s.num)) * ceil_div(s.rank, 16) * 2048;
   w.packed_a = take(packed);
   w.packed_b = take(packed);
   w.part_a = take(static_cast<size_t>(most_items(s)) * s.rank * s.in * sizeof(float));
@@ -865,21 +924,16 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   const BackwardWorkspace w = backward_workspace(s);
   float *up = reinterpret_cast<float *>(ws + w.low);
   uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
-  const Plan plan{reinterpret_cast<int *>(ws + w.order), reinterpret_cast<int *>(ws + w.block_base),
-                  reinterpret_cast<int *>(ws + w.item_base)};
-  const bool wgrad = da != nullptr;
+  const bool wgrad = da != nullptr, in_order = ordered(s.tokens, s.num);
   if (!wgrad && (dx == nullptr || s.tokens == 0)) return;
-  const int per_item = blocks_per_item(s);
-  const int64_t pieces = s.tokens > 0 ? static_cast<int64_t>(s.num) * ceil_div(s.out, 64) : 0, lists = wgrad ? s.num : 0;
-  NVTE_CHECK(lists + pieces <= INT_MAX, "too many adapters: ", s.num);
-  const PrepareArgs prep{ids, static_cast<const uint16_t *>(b), bt, plan, s.tokens, s.out, s.rank, s.num, per_item, static_cast<int>(lists)};
-  hipLaunchKernelGGL(prepare_kernel, dim3(lists + pieces), dim3(1024), 0, stream, prep);
-  NVTE_CHECK_HIP(hipGetLastError());
-  const int64_t blocks = wgrad ? most_blocks(s) : 0;
+  const Plan plan = prepare(s, ids, wgrad || in_order, s.tokens > 0 ? b : nullptr, bt, reinterpret_cast<int *>(ws + w.order),
+                            reinterpret_cast<int *>(ws + w.block_base), reinterpret_cast<int *>(ws + w.item_base), stream);
+  const Plan tiles = in_order ? plan : Plan{};
+  const int64_t blocks = wgrad ? most_blocks(s.tokens, s.num) : 0;
   uint16_t *packed_a = reinterpret_cast<uint16_t *>(ws + w.packed_a), *packed_b = reinterpret_cast<uint16_t *>(ws + w.packed_b);
   if (s.tokens > 0) {
-    shrink<E>(dy, bt, ids, up, s.tokens, s.out, s.rank, s.num, stream);
-    const ExpandArgs e{up, static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(base_grad), scaling, ids,
+    shrink<E>(dy, bt, ids, tiles, up, s.tokens, s.out, s.rank, s.num, stream);
+    const ExpandArgs e{up, static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(base_grad), scaling, ids, tiles,
                        static_cast<uint16_t *>(dx), s.tokens, num_slices(s.tokens, s.out), s.in, s.rank, s.num, 0};
     const PackArgs q{{{up, packed_a, num_slices(s.tokens, s.out)}, {low, packed_b, num_slices(s.tokens, s.in)}}, scaling, plan,
                      s.tokens, s.rank, s.num};
@@ -895,7 +949,7 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   p.tokens = s.tokens;
   p.rank = s.rank;
   p.num = s.num;
-  p.per_item = per_item;
+  p.per_item = blocks_per_item(s);
   p.grad_type = grad_type;
   const int64_t items = most_items(s);
   NVTE_CHECK(items <= 65535, "too many work items: ", items);
@@ -914,25 +968,42 @@ extern "C" {
 
 size_t nvte_amd_lora_num_slices(size_t tokens, size_t features) {
   return api_guard("nvte_amd_lora_num_slices", [&]() -> size_t {
-    NVTE_CHECK(features >= 1 && features <= (1u << 24) && tokens < (1ull << 31) - 64, "bad sizes ", tokens, " and ", features);
+    NVTE_CHECK(features >= 1 && features <= (1u << 24) && tokens <= kMaxTokens, "bad sizes ", tokens, " and ", features);
     return num_slices(static_cast<int64_t>(tokens), static_cast<int>(features));
+  });
+}
+
+size_t nvte_amd_lora_forward_workspace_size(size_t tokens, size_t num_adapters) {
+  return api_guard("nvte_amd_lora_forward_workspace_size", [&]() -> size_t {
+    NVTE_CHECK(tokens <= kMaxTokens && num_adapters <= INT_MAX, "bad sizes ", tokens, " and ", num_adapters);
+    return forward_workspace(static_cast<int64_t>(tokens), static_cast<int>(num_adapters)).bytes;
   });
 }
 
 void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const int *adapter_ids, const float *scaling,
                            const void *base, void *out, float *low, size_t tokens, size_t in_features, size_t out_features,
-                           size_t rank, size_t num_adapters, int dtype, hipStream_t stream) {
+                           size_t rank, size_t num_adapters, int dtype, void *workspace, size_t workspace_bytes,
+                           hipStream_t stream) {
   api_guard("nvte_amd_lora_forward", [&] {
     const Shape s = shape_of(tokens, in_features, out_features, rank, num_adapters, dtype);
     if (s.tokens == 0) return;
     NVTE_CHECK(x && a && b && adapter_ids && out && low, "a required pointer is NULL");
-    const ExpandArgs p{low, static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(base), scaling, adapter_ids,
+    const ForwardWorkspace w = forward_workspace(s.tokens, s.num);
+    NVTE_CHECK(w.bytes == 0 || (workspace != nullptr && workspace_bytes >= w.bytes), "workspace of ", workspace_bytes,
+               " bytes, but ", w.bytes, " are needed");
+    NVTE_CHECK(w.bytes == 0 || aligned16(workspace), "the workspace must be 16-byte aligned");
+    char *ws = static_cast<char *>(workspace);
+    Plan plan{};
+    if (w.bytes != 0)
+      plan = prepare(s, adapter_ids, true, nullptr, nullptr, reinterpret_cast<int *>(ws + w.order),
+                     reinterpret_cast<int *>(ws + w.block_base), reinterpret_cast<int *>(ws + w.item_base), stream);
+    const ExpandArgs p{low, static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(base), scaling, adapter_ids, plan,
                        static_cast<uint16_t *>(out), s.tokens, num_slices(s.tokens, s.in), s.out, s.rank, s.num, 0};
     if (s.type == kNVTEBFloat16) {
-      shrink<bf16_t>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
+      shrink<bf16_t>(x, a, adapter_ids, plan, low, s.tokens, s.in, s.rank, s.num, stream);
       expand<bf16_t>(p, stream);
     } else {
-      shrink<f16_t>(x, a, adapter_ids, low, s.tokens, s.in, s.rank, s.num, stream);
+      shrink<f16_t>(x, a, adapter_ids, plan, low, s.tokens, s.in, s.rank, s.num, stream);
       expand<f16_t>(p, stream);
     }
   });

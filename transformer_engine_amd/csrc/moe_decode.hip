@@ -557,7 +557,7 @@ void run(const Layer &l, const Fc1Args &a, const Fc2Args &b, void *out, hipStrea
   E *o = static_cast<E *>(out);
   const int per_expert = std::min(l.tokens, 2 * l.tokens * l.top_k / l.experts);
   if (per_expert <= 16) launch<W, E, 1, 1, sizeof(W), 4, 2, sizeof(W), 4>(l, a, b, o, stream);
-  else if (per_expert <= 32) launch<W, E, 2, 2, 1, 2, 8, 1, 4>(l, a, b, o, stream);
+  else if (per_expert <= 32) launch<W, E, 2, 2, 1, 4, 8, 1, 4>(l, a, b, o, stream);
   else launch<W, E, 4, 2, 1, 2, 4, 1, 4>(l, a, b, o, stream);
 }
 
@@ -576,7 +576,7 @@ void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, s
     NVTE_CHECK(num_experts >= 1 && num_experts <= kMaxExperts, "number of experts must be 1 to ", kMaxExperts, ", got ", num_experts);
     NVTE_CHECK(top_k >= 1 && top_k <= 64 && top_k <= num_experts, "top_k must be 1 to 64 and at most the number of experts (",
                num_experts, "), got ", top_k);
-    NVTE_CHECK(tokens < (1ull << 31), "too many tokens: ", tokens);
+    NVTE_CHECK(tokens < (1u << 26), "too many tokens: ", tokens);
     if (tokens == 0) return;
     NVTE_CHECK(logits && topk_ids && topk_weights, "a required pointer is NULL");
     auto launch_topk = [&](auto kernel) {

@@ -115,9 +115,12 @@ def lora_forward(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids:
                 raise ValueError(f"out overlaps {name}")
     tokens = ids.numel()
     low = torch.empty((api.nvte_amd_lora_num_slices(tokens, k), tokens, rank), dtype=torch.float32, device=x.device)
+    size = api.nvte_amd_lora_forward_workspace_size(tokens, n)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     api.nvte_amd_lora_forward(x2d.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
                               0 if scaling is None else scaling.data_ptr(), 0 if base is None else base.data_ptr(),
-                              out.data_ptr(), low.data_ptr(), tokens, k, o, rank, n, int(te_dtype(x.dtype)), current_stream_ptr())
+                              out.data_ptr(), low.data_ptr(), tokens, k, o, rank, n, int(te_dtype(x.dtype)),
+                              ws.data_ptr() if size else 0, size, current_stream_ptr())
     saved = LoRASaved(x2d, a, b, ids, scaling, low, tuple(x.shape)) if needs_backward else None
     return out, saved
 
