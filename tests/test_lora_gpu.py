@@ -88,7 +88,10 @@ SHAPES = [  # tokens, in, out, rank, adapters
     (130, 648, 640, 128, 3),
     (333, 128, 136, 100, 2),
     (700, 2056, 264, 12, 40),
+    (520, 96, 104, 4, 300),
     (1500, 520, 1100, 32, 6),
+    (2100, 9, 1030, 128, 4),
+    (1100, 7, 5, 66, 3),
     (4500, 264, 512, 24, 3),
     (4100, 136, 72, 64, 1),
 ]
@@ -116,8 +119,9 @@ def test_no_base_no_scaling_fp32_gradients(dtype):
     assert (y[i < 0] == 0).all() and (dx[i < 0] == 0).all()
 
 
-def test_rows_without_adapter_keep_the_base_bits():
-    x, a, b, i, s, base, dy, gbase = make(50, 64, 96, 8, 2, torch.bfloat16, ids=-1)
+@pytest.mark.parametrize("t", [50, 1300])
+def test_rows_without_adapter_keep_the_base_bits(t):
+    x, a, b, i, s, base, dy, gbase = make(t, 64, 96, 8, 2, torch.bfloat16, ids=-1)
     i[3], i[7], i[20] = 2, 2 ** 31 - 1, -2 ** 31        # all outside [0, 2)
     y, saved = lora_forward(x, a, b, i, s, base=base)
     dx, da, db = lora_backward(dy, saved, base_grad=gbase)
@@ -125,8 +129,9 @@ def test_rows_without_adapter_keep_the_base_bits():
     assert (da == 0).all() and (db == 0).all()
 
 
-def test_adapters_without_tokens_get_zero_gradients_over_old_memory():
-    x, a, b, i, s, base, dy, _ = make(40, 72, 80, 8, 6, torch.float16, ids=4)
+@pytest.mark.parametrize("t", [40, 1000])
+def test_adapters_without_tokens_get_zero_gradients_over_old_memory(t):
+    x, a, b, i, s, base, dy, _ = make(t, 72, 80, 8, 6, torch.float16, ids=4)
     torch.full((6, 8, 72), float("nan"), dtype=torch.float16, device="cuda")   # freed at once: what the allocator may hand out
     y, saved = lora_forward(x, a, b, i, s, base=base)
     _, da, db = lora_backward(dy, saved)
@@ -196,6 +201,32 @@ def test_strided_inputs_leading_dims_and_in_place_output():
     buf = base.clone()
     y, saved = lora_forward(x, a, b, i, s, base=buf, out=buf, needs_backward=False)
     assert y is buf and saved is None and torch.equal(buf, ref)
+
+
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("o", [96, 1029, 2052])
+def test_in_place_of_a_large_batch(o, n):
+    x, a, b, i, s, base, _, _ = make(1400, 64, o, 8, n, torch.bfloat16, seed=17)
+    ref, _ = lora_forward(x, a, b, i, s, base=base)
+    buf = base.clone()
+    lora_forward(x, a, b, i, s, base=buf, out=buf)
+    assert torch.equal(buf, ref)
+    none, _ = lora_forward(x, a, b, i, s)
+    zero, _ = lora_forward(x, a, b, i, s, base=torch.zeros_like(base))
+    assert torch.equal(none, zero) and (none[i < 0] == 0).all()
+
+
+def test_the_order_of_the_tokens_does_not_change_a_row():
+    """A large mixed batch, its tokens put in another order: the same rows, and gradients within their bounds."""
+    args = make(3000, 264, 392, 16, 20, torch.bfloat16, seed=18)
+    x, a, b, i, s, base, dy, gbase = args
+    p = torch.randperm(3000, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    y0, saved = lora_forward(x, a, b, i, s, base=base)
+    dx0, _, _ = lora_backward(dy, saved, base_grad=gbase)
+    y1, saved = lora_forward(x[p], a, b, i[p], s, base=base[p])
+    dx1, da1, db1 = lora_backward(dy[p], saved, base_grad=gbase[p])
+    assert torch.equal(y0[p], y1) and torch.equal(dx0[p], dx1)
+    check_all(args, y0, dx0, da1, db1)
 
 
 @pytest.mark.parametrize("off", [1, 4])
@@ -294,8 +325,9 @@ def test_autograd_matches_the_bare_passes():
     assert torch.equal(xs[1].grad, da)
 
 
-def test_captured_and_replayed():
-    x, a, b, i, s, base, dy, gbase = make(300, 264, 392, 16, 5, torch.bfloat16, seed=14)
+@pytest.mark.parametrize("t", [1, 300, 1300])
+def test_captured_and_replayed(t):
+    x, a, b, i, s, base, dy, gbase = make(t, 264, 392, 16, 5, torch.bfloat16, seed=14)
     def step():
         y, saved = lora_forward(x, a, b, i, s, base=base)
         return (y, *lora_backward(dy, saved, base_grad=gbase))

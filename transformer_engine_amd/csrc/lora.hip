@@ -215,7 +215,7 @@ struct ExpandArgs {
 
 // A wave's step is 128 columns: operand f holds the columns c0 + 8 n + f, n = 0 .. 15.  D then leaves lane (n, lane group q), register i
 // with the eight neighbours c0 + 8 n + 0 .. 7 of token 4 q + i over f, so that each of the four stores of a step writes 256 contiguous
-// bytes of four tokens (tokens along the lanes instead: 64 bytes of sixteen, 119 against XX us at 8192 x 14336, rank 32).
+// bytes of four tokens (tokens along the lanes instead, 64 bytes of sixteen a store: 119 against 103 us at 8192 x 14336, rank 32).
 // Ends: a chunk of eight columns past the last takes the last eight, and its lanes write only what is theirs.  Likewise the ranks:
 // `slot_rank` says which rank operand slot s stands for (-1: none, zero in the rank vector), so that the pool is always read in whole
 // eights.  A rank past the last (RMAJOR) reads the last one again and meets such a zero.
@@ -769,9 +769,10 @@ int64_t tiles_of(const Plan &plan, int64_t tokens, int num, int size) {
   return plan.order != nullptr ? most_blocks(tokens, num) * kBlock / size : static_cast<int64_t>(ceil_div(tokens, size));
 }
 
-// Tokens are put in order of their adapters first where tiles would otherwise walk through many: a batch of 8192 with 64 adapters in any
-// order took 1356 us without and XX us with it; one whose requests lie back to back pays the extra launch (XX us at 2931 tokens).
-bool ordered(int64_t tokens, int num) { return tokens >= 1024 && num > 1 && num <= kMaxAdapters; }
+// Tokens are put in order of their adapters first where tiles would otherwise walk through many.  In any order, 8192 x (8192 -> 14336) with 64
+// adapters of rank 8 took 1356 us without and 219 us with it, 600 x (4096 -> 4096) with 32 of rank 16 46 and 26 us; a batch whose
+// requests lie back to back pays the extra launch (23 and 28 us at the latter size), and below 512 tokens both orders lose.
+bool ordered(int64_t tokens, int num) { return tokens >= 512 && num > 1 && num <= kMaxAdapters; }
 
 template <typename E, int RT, int MT, int NW, int U, bool SMALL = false>
 void launch_shrink(const ShrinkArgs &p, int slices, hipStream_t stream) {
