@@ -123,9 +123,11 @@ def test_no_base_no_scaling_fp32_gradients(dtype):
 def test_rows_without_adapter_keep_the_base_bits(t):
     x, a, b, i, s, base, dy, gbase = make(t, 64, 96, 8, 2, torch.bfloat16, ids=-1)
     i[3], i[7], i[20] = 2, 2 ** 31 - 1, -2 ** 31        # all outside [0, 2)
+    base[5, :50], gbase[6, 10:] = -0.0, -0.0
     y, saved = lora_forward(x, a, b, i, s, base=base)
     dx, da, db = lora_backward(dy, saved, base_grad=gbase)
-    assert torch.equal(y, base) and torch.equal(dx, gbase)
+    bits = lambda v: v.view(torch.int16)
+    assert torch.equal(bits(y), bits(base)) and torch.equal(bits(dx), bits(gbase))
     assert (da == 0).all() and (db == 0).all()
 
 

@@ -394,7 +394,8 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
           const E *old = reinterpret_cast<const E *>(&base[m][i]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) narrow(widen(old[k]) + res[m][k][i], o[k]);
-          const u32x4 bits = *reinterpret_cast<const u32x4 *>(o);
+          // a token without an adapter keeps its bits (-0 + 0 would be +0)
+          const u32x4 sum = *reinterpret_cast<const u32x4 *>(o), bits = my_id[m][i] < 0 ? base[m][i] : sum;
           if (c + 8 <= p.features) {
             store8(to + c, bits);
           } else if (c < p.features) {
@@ -453,22 +454,27 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t stretch = ((p.tokens + 15) / 16 + 63) / 64 * 64, from = wave * stretch;
   const int64_t to = min(from + stretch, p.tokens);
-  // its adapter, num for none; -1 past the stretch
-  auto id_of = [&](int64_t t) {
-    if (t >= to) return -1;
-    const int id = p.ids[t];
-    return id >= 0 && id < p.num ? id : p.num;
+  // the adapters of 256 tokens (num: none, -1: past the stretch), four loads on their way at once
+  auto ids_of = [&](int64_t t0, int (&id)[4]) {
+    int raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = p.ids[min(t0 + 64 * i + lane, p.tokens - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = t0 + 64 * i + lane >= to ? -1 : raw[i] >= 0 && raw[i] < p.num ? raw[i] : p.num;
   };
   for (int i = threadIdx.x; i <= p.num; i += 1024) hist[i] = 0;
   __syncthreads();
-  for (int64_t t0 = from; t0 < to; t0 += 64) {
-    const int id = id_of(t0 + lane);
-    for (uint64_t left = __ballot(id >= 0); left != 0;) {  // one addition per distinct id: a run would queue up on one address
-      const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-      const uint64_t same = __ballot(id == cur);
-      left &= ~same;
-      if (lane == 0) atomicAdd(&hist[cur], __popcll(same));
-    }
+  for (int64_t t0 = from; t0 < to; t0 += 256) {
+    int id[4];
+    ids_of(t0, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      for (uint64_t left = __ballot(id[i] >= 0); left != 0;) {  // one addition per distinct id: a run would queue up on one address
+        const int cur = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(left));
+        const uint64_t same = __ballot(id[i] == cur);
+        left &= ~same;
+        if (lane == 0) atomicAdd(&hist[cur], __popcll(same));
+      }
   }
   __syncthreads();
   int blocks = 0, items = 0;
@@ -488,20 +494,30 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   if (mine == 0) return;
   int *order = p.order + static_cast<int64_t>(blocks) * kBlock;
   int count = 0;
-  for (int64_t t0 = from; t0 < to; t0 += 64) count += __popcll(__ballot(id_of(t0 + lane) == a));
+  for (int64_t t0 = from; t0 < to; t0 += 256) {
+    int id[4];
+    ids_of(t0, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) count += __popcll(__ballot(id[i] == a));
+  }
   __syncthreads();
   if (lane == 0) scratch[wave] = count;
   __syncthreads();
   int at = 0;
   for (int w = 0; w < wave; ++w) at += scratch[w];
-  for (int64_t t0 = from; t0 < to; t0 += 64) {
-    const bool hit = id_of(t0 + lane) == a;
-    const uint64_t m = __ballot(hit);
-    const int slot = at + __popcll(m & ((1ull << lane) - 1)), t = static_cast<int>(t0) + lane;
-    if (hit) order[slot] = t;
-    if (hit && slot == mine - 1)
-      for (int i = mine; i < my_blocks * kBlock; ++i) order[i] = t | INT_MIN;
-    at += __popcll(m);
+  for (int64_t t0 = from; t0 < to; t0 += 256) {
+    int id[4];
+    ids_of(t0, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool hit = id[i] == a;
+      const uint64_t m = __ballot(hit);
+      const int slot = at + __popcll(m & ((1ull << lane) - 1)), t = static_cast<int>(t0) + 64 * i + lane;
+      if (hit) order[slot] = t;
+      if (hit && slot == mine - 1)
+        for (int k = mine; k < my_blocks * kBlock; ++k) order[k] = t | INT_MIN;
+      at += __popcll(m);
+    }
   }
 }
 
