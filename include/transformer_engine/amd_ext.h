@@ -111,7 +111,8 @@ void nvte_amd_clip_by_sum_of_squares(const void *const *grads, void *const *outs
  * [num_adapters] fp32 or NULL (1); base NULL = zero, or out itself.  rank 1 to 128, any feature sizes.
  *   low[t] = a[id] x[t]        out[t] = base[t] + scaling[id] b[id] low[t]
  * low [nvte_amd_lora_num_slices(tokens, in), tokens, rank] fp32: partial sums of the rank vectors, which the backward pass reads
- * (rows without an adapter are not written).  A non-finite weight or activation makes its own rows non-finite and no other. */
+ * (rows without an adapter are not written).  A non-finite weight or activation makes its own rows non-finite and no other; where
+ * the sum would be Inf it may be NaN. */
 size_t nvte_amd_lora_num_slices(size_t tokens, size_t features);
 size_t nvte_amd_lora_forward_workspace_size(size_t tokens, size_t num_adapters);   /* 0: workspace may be NULL */
 void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const int *adapter_ids, const float *scaling,
@@ -136,7 +137,8 @@ void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, s
 /* out[t] = sum_j topk_weights[t, j] w_fc2[e] (silu(w_fc1[e][:ffn] x[t]) * (w_fc1[e][ffn:] x[t])), e = topk_ids[t, j]; an id
  * outside [0, num_experts) adds nothing.  x, out [tokens, hidden] bf16 or fp16; w_fc1 [num_experts, 2 ffn, hidden] and w_fc2
  * [num_experts, hidden, ffn] of the same dtype, or FP8 E4M3 with one fp32 scale_inv per expert.  Up to 256 tokens, top_k up to
- * 64, tokens * top_k up to 4096.  out must not overlap an input. */
+ * 64, tokens * top_k up to 4096.  out must not overlap an input.  Non-finite values as above: those of one token or expert stay
+ * with the tokens that meet them. */
 size_t nvte_amd_moe_forward_workspace_size(size_t tokens, size_t top_k, size_t num_experts, size_t hidden, size_t ffn);
 void nvte_amd_moe_forward(const void *x, const void *w_fc1, const void *w_fc2, const float *fc1_scale_inv,
                           const float *fc2_scale_inv, const int *topk_ids, const float *topk_weights, void *out,

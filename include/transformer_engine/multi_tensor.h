@@ -1,7 +1,8 @@
 /* Multi-tensor kernels of the FP8 weight-update path: one launch walks lists of tensors.
  * Replaces the part of reference .../include/transformer_engine/multi_tensor.h that an
  * "FP8 primary weights" optimizer step calls; the other fused optimizers
- * (plain Adam, SGD, L2 norm) are outside the FP8 linear path and are not provided.
+ * (plain Adam, SGD, L2 norm) are outside the FP8 linear path and are not provided; the norm of all
+ * gradients together and clipping by it are in amd_ext.h (nvte_amd_grad_norm, nvte_amd_clip_grad_norm).
  *
  * tensor_lists is [num_tensor_lists][num_tensors_per_list]; list 0 gives the element counts and
  * the data lists must match it element for element.  chunk_size is the number of elements one

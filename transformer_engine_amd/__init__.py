@@ -11,7 +11,10 @@ Package layout (only what the path needs):
   grouped.py / grouped_linear.py  grouped (MoE) tensors, quantize and GEMM with device-side splits
   normalization.py  LayerNorm / RMSNorm with fused FP8 output (LayerNormLinear lives in linear.py)
   activation.py  plain / gated activations fused with the FP8 cast, transpose and dbias
-  weight_update.py  sharded master weights -> FP8 primary weights (multi-tensor kernels, MXFP8 shard cast)
+  weight_update.py  sharded master weights -> FP8 primary weights (multi-tensor kernels, MXFP8 shard cast),
+             global gradient norm and clipping
+  lora.py    low-rank adapters of many requests beside a shared projection (fwd + bwd), LoRALinear
+  moe.py     router selection and a whole expert layer for a few tokens (decode)
 """
 from ._lib import NVTEError, api, version  # noqa: F401
 from .tensor import (DType, Float8CurrentScalingQuantizer, Float8Quantizer, Float8Tensor,  # noqa: F401

@@ -73,6 +73,10 @@ __device__ __forceinline__ TileToken tile_token(const Plan &plan, const int *ids
 
 // ====================================================================================
 // shrink: out[slice][t][j] = sum over the slice's k of in[t][k] * pool[a][j][k]
+// Reads every activation once (2 T K bytes); tokens are the rows of the product, ranks its columns, both operands come from memory in
+// the matrix layout (eight consecutive k per lane), so LDS only joins the waves' sums.  8192 x 4096, rank 32: 21 us (3.2 TB/s);
+// 8192 x 14336 right after the pass that wrote it: 74 us, of which the writing back of that pass's lines is part; 96 x 4096 with 48
+// adapters of rank 16 (12.6 MB of pool, each adapter read by about two tiles): 6.0 us.
 // ====================================================================================
 struct ShrinkArgs {
   const uint16_t *in, *pool;
@@ -201,6 +205,8 @@ __device__ __forceinline__ float sum_slices(const float *p, int slices, int64_t 
 // ====================================================================================
 // expand: out[t][c] = base[t][c] + s_a sum_j (sum over slices of low[slice][t][j]) * w(c, j)
 // w(c, j) = pool[a][c][j], or pool[a][j][c] (RMAJOR)
+// Reads and writes 2 T O bytes each, which bounds it: 8192 x 14336, rank 32: 104 us (4.5 TB/s).  A decode tile is bound by its adapters
+// instead: 96 x 14336 with 48 of rank 16 (22 MB of pool, read about twice) 15 us.
 // ====================================================================================
 struct ExpandArgs {
   const float *low;
@@ -426,7 +432,8 @@ __global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_kernel(ExpandArgs
 // prepare: the lists of a Plan, and where each adapter's work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to
 // [rank][features].
 // One workgroup per adapter counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged; its sixteen waves own
-// consecutive stretches of the tokens.
+// consecutive stretches of the tokens.  Three dependent walks of the ids: latency (2931 tokens 6.4 us, 8192 tokens and a 32 x 14336
+// transpose 8.4 us).
 // ====================================================================================
 struct PrepareArgs {
   const int *ids;
@@ -595,6 +602,10 @@ __global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_pack_kernel(Expan
 
 // ====================================================================================
 // wgrad: one work item's sums over its tokens of w[t] (x) z[t]: dA with z = x, dB (transposed) with z = dy
+// Reads every activation of x and dy once per 64 ranks, rows of 256 bytes, and turns 8 x 8 blocks round in registers (the tokens are k
+// here); the rank vectors come packed as operands, shared by all column groups out of L2.  8192 tokens, 4096 + 14336 columns, rank 32:
+// 58 us (5.2 TB/s); with rank vectors put together in the kernel 117 us, 64 columns per wave 69 us.  A work item's partial sums go to
+// `join` in fp32 (8 us there): items add up in a fixed order, no atomics.
 // ====================================================================================
 struct WgradSide {
   const uint16_t *z;       // activations [tokens][features]
@@ -764,7 +775,8 @@ Shape shape_of(size_t tokens, size_t in, size_t out, size_t rank, size_t num, in
 }
 
 // Few tokens leave most CUs without a tile, so the features are cut into slices (a multiple of 64, at least 512) until about
-// 768 workgroups run, three per CU; whoever reads the rank vectors adds the slices.
+// 768 workgroups run, three per CU; whoever reads the rank vectors adds the slices.  From 4096 tokens on a workgroup takes 32 tokens for one
+// reading of the adapter (8192 x 14336, rank 32: 74 against 86 us with 16; 2048 x 4096, rank 16, within 2 %).
 bool many_tokens(int64_t tokens) { return tokens >= 4096; }
 int slice_of(int64_t tokens, int features) {
   const int64_t tiles = std::max<int64_t>(1, ceil_div(tokens, many_tokens(tokens) ? 32 : 16));
@@ -773,7 +785,8 @@ int slice_of(int64_t tokens, int features) {
 }
 int num_slices(int64_t tokens, int features) { return static_cast<int>(ceil_div(features, slice_of(tokens, features))); }
 
-// a decode tile's adapters go to workgroups of their own while there are too few of them
+// A decode tile's adapters go to workgroups of their own while there are too few of them: expand of 96 tokens, 48 adapters takes 15 us
+// with up to 768, 17.5 with 448, 18.4 with 1024 (a second round of workgroups).
 int phases_of(int64_t workgroups, int64_t tokens, int num) {
   const int64_t most = std::min<int64_t>(std::min<int64_t>(num, tokens), 16);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 768 / workgroups)));
@@ -818,7 +831,10 @@ void shrink(const void *in, const void *pool, const int *ids, const Plan &plan, 
   }
 }
 
-// runs launch(KT, MT, SMALL) as integral constants: 32 ranks per operand, 16 tokens per tile
+// Runs launch(KT, MT, SMALL) as integral constants: 32 ranks per operand, 16 tokens per tile.  32 tokens share one reading of the adapter
+// from 1024 tokens on: whole forward passes in us, with 32 / with 16, 1024 x 4096 x 4096 rank 16 24.5 / 25.0, 2048 likewise 31.7 / 35.4,
+// 4096 x 8192 x 8192 rank 32 70.5 / 75.1, 8192 x 4096 x 14336 rank 64 202 / 227; the other way at rank 64 of 4096 x 4096 x 4096 59 / 56 and
+// four adapters of rank 16 in 8192 x 4096 x 14336 167 / 159.
 template <typename Launch>
 void expand_variant(int rank, int64_t tokens, bool small_features, bool small_rank, Launch &&launch) {
   typedef std::integral_constant<int, 1> One;
@@ -832,7 +848,7 @@ void expand_variant(int rank, int64_t tokens, bool small_features, bool small_ra
   else launch(Four(), One(), std::false_type());
 }
 
-// columns per workgroup: 512 until there are about 1024 workgroups
+// columns per workgroup: 512 (a step of its four waves) until there are about 1024 workgroups
 int columns_of(int64_t tiles, int features) {
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(features, 512), 1024 / tiles));
   return static_cast<int>(round_up(ceil_div(features, static_cast<size_t>(want)), 512));

@@ -7,7 +7,8 @@
 // rounded bf16 term alone would add an error as large as the final rounding of a bf16 result, and these kernels are bound
 // by memory, so the second matrix instruction is free.  fp16 operands that meet such a pair are split the same way (11 bits
 // fit two bf16 terms exactly), which keeps bf16's exponent range for products of small gradients; the lo * lo term
-// (2^-17 of a product) is left out.  Non-finite values split as hi = x, lo = 0.
+// (2^-17 of a product) is left out.  Non-finite values split as hi = x, lo = 0: a sum with one stays non-finite, but an Inf may meet the
+// other operand's zero or opposite second term and become NaN.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -94,9 +95,9 @@ __device__ __forceinline__ u32x4 load8_once(const uint16_t *p) {
 }
 __device__ __forceinline__ void store8(uint16_t *p, u32x4 v) { *reinterpret_cast<u32x4_any *>(p) = v; }
 // The ends of rows whose length is no multiple of the step: a lane whose eight elements would reach past the end takes the last
-// eight instead and, where they are summed, has the `skip` that its neighbour holds already set to zero.  This keeps the kernels
-// small (instruction cache misses cost these short kernels more than the arithmetic: an expand kernel with element-wise ends had 32 KiB
-// of code and ran 18 us on 6 MB).
+// eight instead and, where they are summed, has the `skip` that its neighbour holds already set to zero (in one operand at
+// least).  This keeps the kernels small (instruction cache misses cost these short kernels more than the arithmetic: an expand kernel
+// with element-wise ends had 32 KiB of code and ran 18 us on 6 MB).
 __device__ __forceinline__ u32x4 without_head(u32x4 v, int skip) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) v[w] &= skip <= 2 * w ? 0xFFFFFFFFu : skip <= 2 * w + 1 ? 0xFFFF0000u : 0u;

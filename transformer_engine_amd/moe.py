@@ -4,8 +4,9 @@
     out[t] = sum_j weights[t, j] * W2[e] (silu(W1[e, :F] x[t]) * (W1[e, F:] x[t])),   e = ids[t, j]
 
 The experts' weights are read once per batch and the routing stays on the device, as in ``grouped``: nothing is sorted or padded on
-the host, and the three launches of ``moe_forward`` can be captured into a HIP graph.  Batches of more than 256 tokens are
-``grouped_linear``'s.  The gate order is that of ``activation("swiglu", ...)``: activation half first.
+the host, and the three launches of ``moe_forward`` can be captured into a HIP graph.  Batches of more than 256 tokens and training
+are ``grouped_linear``'s: there is no backward pass here, results carry no gradient.  The gate order is that of
+``activation("swiglu", ...)``: activation half first.
 """
 from __future__ import annotations
 
@@ -25,7 +26,8 @@ def moe_topk(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Tupl
     """Softmax over the last dim of ``logits`` [tokens, experts] (fp32 / bf16 / fp16, up to 1024 experts) and its ``top_k`` largest.
 
     Returns ``(ids int32 [tokens, top_k], weights fp32 [tokens, top_k])`` in falling order; equal logits go to the lowest index,
-    NaN ranks last.  ``renormalize`` divides a token's weights by their sum."""
+    NaN ranks last (and makes its token's weights NaN, except with ``renormalize`` where it is not chosen itself).  ``renormalize``
+    divides a token's weights by their sum."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
