@@ -37,22 +37,15 @@ __device__ __forceinline__ int valid_id(const int *ids, int64_t t, int64_t token
 constexpr int kBlock = 32;
 
 // The tokens of every adapter in rising order, then those without one; each list padded to whole blocks with its last token, marked
-// by the sign bit (see `prepare`).
+// by the sign bit (see `prepare`).  Whatever a workgroup asks of it is one load away: these kernels are short, and a search through the
+// adapters' first blocks was a chain of loads at the head of each.
 struct Plan {
-  const int *order;       // [most_blocks * 32]; null: tokens are taken as they come
-  const int *block_base;  // [num + 2] first block of every adapter in `order`, of the rest, and the end
-  const int *item_base;   // [num + 1] first work item of every adapter
+  int *order;      // [most_blocks * 32]; null: tokens are taken as they come
+  int *owner;      // [most_blocks] each block's adapter, num: none
+  int *ends;       // [2] blocks with an adapter, all blocks
+  int *item_base;  // [num + 1] first work item of every adapter, and the end
+  int2 *items;     // [most_items] each work item's first and last + 1 block; null: not wanted, nor item_base
 };
-
-// the adapter whose range of `base` holds `i` (one without tokens holds none)
-__device__ __forceinline__ int owner_of(const int *base, int num, int i) {
-  int a = 0;
-  for (int hi = num; hi - a > 1;) {
-    const int mid = (a + hi) >> 1;
-    if (base[mid] <= i) a = mid; else hi = mid;
-  }
-  return a;
-}
 
 // a lane's token of a tile of 16 MT, and its adapter: -1 none, -2 no token
 struct TileToken {
@@ -66,8 +59,9 @@ __device__ __forceinline__ TileToken tile_token(const Plan &plan, const int *ids
     return {min(t, tokens - 1), lane < size && t < tokens ? valid_id(ids, t, tokens, num) : -2};
   }
   const int block = static_cast<int>(tile * size / kBlock);
-  if (block >= plan.block_base[num + 1]) return {0, -2};
-  const int v = plan.order[tile * size + min(lane, size - 1)], a = owner_of(plan.block_base, num + 1, block);
+  // past the end they are whatever memory held
+  const int end = plan.ends[1], v = plan.order[tile * size + min(lane, size - 1)], a = plan.owner[block];
+  if (block >= end) return {0, -2};
   return {v & INT_MAX, lane < size && v >= 0 ? (a < num ? a : -1) : -2};
 }
 
@@ -432,14 +426,14 @@ __global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_kernel(ExpandArgs
 // prepare: the lists of a Plan, and where each adapter's work items of `per_item` blocks begin.  And B[a] [features][rank] transposed to
 // [rank][features].
 // One workgroup per adapter counts all ids for itself (T * 4 bytes out of L2), so nothing is exchanged; its sixteen waves own
-// consecutive stretches of the tokens.  Three dependent walks of the ids: latency (2931 tokens 6.4 us, 8192 tokens and a 32 x 14336
-// transpose 8.4 us).
+// consecutive stretches of the tokens.  Two dependent walks of the ids: latency (2931 tokens 6.0 us, 8192 tokens and a 32 x 14336
+// transpose 8.0 us).
 // ====================================================================================
 struct PrepareArgs {
   const int *ids;
   const uint16_t *pool;
   uint16_t *transposed;
-  int *order, *block_base, *item_base;
+  Plan plan;
   int64_t tokens;
   int features, rank, num, per_item, lists;  // lists: workgroups of the first part, num + 1 or none
 };
@@ -471,17 +465,19 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   };
   for (int i = threadIdx.x; i <= p.num; i += 1024) hist[i] = 0;
   __syncthreads();
+  int id[4], count = 0;
   for (int64_t t0 = from; t0 < to; t0 += 256) {
-    int id[4];
     ids_of(t0, id);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      count += __popcll(__ballot(id[i] == a));
       for (uint64_t left = __ballot(id[i] >= 0); left != 0;) {  // one addition per distinct id: a run would queue up on one address
         const int cur = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(left));
         const uint64_t same = __ballot(id[i] == cur);
         left &= ~same;
         if (lane == 0) atomicAdd(&hist[cur], __popcll(same));
       }
+    }
   }
   __syncthreads();
   int blocks = 0, items = 0;
@@ -494,27 +490,25 @@ __device__ void list_tokens(const PrepareArgs &p, int a, int *hist, int *scratch
   items = sum_1024(items, scratch);
   const int mine = hist[a], my_blocks = (mine + kBlock - 1) / kBlock;
   if (threadIdx.x == 0) {
-    p.block_base[a] = blocks;
-    p.item_base[a] = items;  // that of a == num is the end
-    if (a == p.num) p.block_base[a + 1] = blocks + my_blocks;
+    if (p.plan.items != nullptr) p.plan.item_base[a] = items;  // that of a == num is the end
+    if (a == p.num) {
+      p.plan.ends[0] = blocks;
+      p.plan.ends[1] = blocks + my_blocks;
+    }
   }
   if (mine == 0) return;
-  int *order = p.order + static_cast<int64_t>(blocks) * kBlock;
-  int count = 0;
-  for (int64_t t0 = from; t0 < to; t0 += 256) {
-    int id[4];
-    ids_of(t0, id);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) count += __popcll(__ballot(id[i] == a));
-  }
-  __syncthreads();
+  for (int b = threadIdx.x; b < my_blocks; b += 1024) p.plan.owner[blocks + b] = a;
+  if (p.plan.items != nullptr && a < p.num)
+    for (int i = threadIdx.x, last = (my_blocks + p.per_item - 1) / p.per_item; i < last; i += 1024)
+      p.plan.items[items + i] = int2{blocks + i * p.per_item, blocks + min((i + 1) * p.per_item, my_blocks)};
+  int *order = p.plan.order + static_cast<int64_t>(blocks) * kBlock;
+  __syncthreads();  // the last sum is read
   if (lane == 0) scratch[wave] = count;
   __syncthreads();
   int at = 0;
   for (int w = 0; w < wave; ++w) at += scratch[w];
   for (int64_t t0 = from; t0 < to; t0 += 256) {
-    int id[4];
-    ids_of(t0, id);
+    if (stretch > 256) ids_of(t0, id);  // else they are still there
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool hit = id[i] == a;
@@ -570,8 +564,8 @@ struct PackArgs {
 };
 
 __device__ __forceinline__ void pack_block(const PackArgs &p, const PackSide &side, int block) {
-  if (block >= p.plan.block_base[p.num]) return;
-  const float scale = p.scaling != nullptr ? p.scaling[owner_of(p.plan.block_base, p.num, block)] : 1.f;
+  if (block >= p.plan.ends[0]) return;
+  const float scale = p.scaling != nullptr ? p.scaling[p.plan.owner[block]] : 1.f;
   const int tiles = (p.rank + 15) / 16;
   uint16_t *out = side.packed + static_cast<int64_t>(block) * tiles * 1024;
   // neighbouring threads take neighbouring ranks of one token
@@ -618,7 +612,7 @@ struct WgradArgs {
   WgradSide side[2];
   Plan plan;
   int64_t tokens;
-  int rank, num, per_item, grad_type;
+  int rank, num, grad_type;
 };
 
 struct WgradTokens {  // a lane's eight tokens of a block
@@ -668,9 +662,7 @@ __global__ __launch_bounds__(256, RT <= 2 ? 2 : 1) void wgrad_kernel(WgradArgs p
   const WgradSide side = second ? p.side[1] : p.side[0];
   const int c0 = (blockIdx.x - (second ? p.side[0].groups : 0)) * 512 + wave * 128;
   if (c0 >= side.features) return;
-  const int a = __builtin_amdgcn_readfirstlane(owner_of(p.plan.item_base, p.num, item));
-  const int first = __builtin_amdgcn_readfirstlane(p.plan.block_base[a] + (item - p.plan.item_base[a]) * p.per_item);
-  const int last = __builtin_amdgcn_readfirstlane(min(first + p.per_item, p.plan.block_base[a + 1]));
+  const int first = __builtin_amdgcn_readfirstlane(p.plan.items[item].x), last = __builtin_amdgcn_readfirstlane(p.plan.items[item].y);
   // a lane past the last column computes the last eight once more, and stores the same values
   const int c = min(c0 + 8 * (lane & 15), max(side.features - 8, 0));
   const int rank_tiles = (p.rank + 15) / 16, j0 = blockIdx.z * 4;
@@ -903,51 +895,66 @@ int64_t most_items(const Shape &s) {
 }
 
 // one launch: the lists, if wanted, and B transposed, if given
-Plan prepare(const Shape &s, const int *ids, bool lists, const void *b, uint16_t *transposed, int *order, int *block_base,
-             int *item_base, hipStream_t stream) {
+void prepare(const Shape &s, const int *ids, const Plan &plan, bool lists, const void *b, uint16_t *transposed, hipStream_t stream) {
   const int64_t pieces = b != nullptr ? static_cast<int64_t>(s.num) * ceil_div(s.out, 64) : 0, first = lists ? s.num + 1 : 0;
   NVTE_CHECK(first + pieces < (1 << 22), "too many adapters to transpose: ", s.num);
-  const PrepareArgs p{ids, static_cast<const uint16_t *>(b), transposed, order, block_base, item_base, s.tokens, s.out, s.rank, s.num,
-                      blocks_per_item(s), static_cast<int>(first)};
+  const PrepareArgs p{ids, static_cast<const uint16_t *>(b), transposed, plan, s.tokens, s.out, s.rank, s.num, blocks_per_item(s),
+                      static_cast<int>(first)};
   hipLaunchKernelGGL(prepare_kernel, dim3(first + pieces), dim3(1024), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
-  return {order, block_base, item_base};
 }
 
+struct Space {  // offsets into a workspace
+  size_t at = 0;
+  size_t take(size_t bytes) {
+    const size_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  }
+};
+
 struct ForwardWorkspace {
-  size_t order, block_base, item_base, bytes;
+  size_t order, owner, ends, bytes;
+  Plan plan(char *ws) const {
+    return {reinterpret_cast<int *>(ws + order), reinterpret_cast<int *>(ws + owner), reinterpret_cast<int *>(ws + ends), nullptr,
+            nullptr};
+  }
 };
 ForwardWorkspace forward_workspace(int64_t tokens, int num) {
   if (!ordered(tokens, num)) return {};
   ForwardWorkspace w{};
-  w.block_base = round_up(most_blocks(tokens, num) * kBlock * sizeof(int), 256);
-  w.item_base = w.block_base + round_up((num + 2) * sizeof(int), 256);
-  w.bytes = w.item_base + round_up((num + 1) * sizeof(int), 256);
+  Space space;
+  w.order = space.take(most_blocks(tokens, num) * kBlock * sizeof(int));
+  w.owner = space.take(most_blocks(tokens, num) * sizeof(int));
+  w.ends = space.take(2 * sizeof(int));
+  w.bytes = space.at;
   return w;
 }
 
 struct BackwardWorkspace {
-  size_t low, transposed, order, block_base, item_base, packed_a, packed_b, part_a, part_b, bytes;
+  size_t low, transposed, order, owner, ends, item_base, items, packed_a, packed_b, part_a, part_b, bytes;
+  Plan plan(char *ws) const {
+    return {reinterpret_cast<int *>(ws + order), reinterpret_cast<int *>(ws + owner), reinterpret_cast<int *>(ws + ends),
+            reinterpret_cast<int *>(ws + item_base), reinterpret_cast<int2 *>(ws + items)};
+  }
 };
 BackwardWorkspace backward_workspace(const Shape &s) {
   BackwardWorkspace w{};
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += round_up(bytes, 256);
-    return here;
-  };
+  Space space;
+  auto take = [&](size_t bytes) { return space.take(bytes); };
   w.low = take(static_cast<size_t>(num_slices(s.tokens, s.out)) * s.tokens * s.rank * sizeof(float));
   w.transposed = take(static_cast<size_t>(s.num) * s.rank * s.out * 2);
   w.order = take(most_blocks(s.tokens, s.num) * kBlock * sizeof(int));
-  w.block_base = take((s.num + 2) * sizeof(int));
-  w.item_base = take((s.num + 1) * sizeof(int));
+  w.owner = take(most_blocks(s.tokens, s.num) * sizeof(int));
+  w.ends = take(2 * sizeof(int));
+  w.item_base = take((static_cast<size_t>(s.num) + 1) * sizeof(int));
+  w.items = take(most_items(s) * sizeof(int2));
   const size_t packed = static_cast<size_t>(most_blocks(s.tokens, s.num)) * ceil_div(s.rank, 16) * 2048;
   w.packed_a = take(packed);
   w.packed_b = take(packed);
   w.part_a = take(static_cast<size_t>(most_items(s)) * s.rank * s.in * sizeof(float));
   w.part_b = take(static_cast<size_t>(most_items(s)) * s.rank * s.out * sizeof(float));
-  w.bytes = at;
+  w.bytes = space.at;
   return w;
 }
 
@@ -959,8 +966,8 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
   const bool wgrad = da != nullptr, in_order = ordered(s.tokens, s.num);
   if (!wgrad && (dx == nullptr || s.tokens == 0)) return;
-  const Plan plan = prepare(s, ids, wgrad || in_order, s.tokens > 0 ? b : nullptr, bt, reinterpret_cast<int *>(ws + w.order),
-                            reinterpret_cast<int *>(ws + w.block_base), reinterpret_cast<int *>(ws + w.item_base), stream);
+  const Plan plan = w.plan(ws);
+  prepare(s, ids, plan, wgrad || in_order, s.tokens > 0 ? b : nullptr, bt, stream);
   const Plan tiles = in_order ? plan : Plan{};
   const int64_t blocks = wgrad ? most_blocks(s.tokens, s.num) : 0;
   uint16_t *packed_a = reinterpret_cast<uint16_t *>(ws + w.packed_a), *packed_b = reinterpret_cast<uint16_t *>(ws + w.packed_b);
@@ -982,7 +989,6 @@ void backward(const Shape &s, const void *x, const void *dy, const void *a, cons
   p.tokens = s.tokens;
   p.rank = s.rank;
   p.num = s.num;
-  p.per_item = blocks_per_item(s);
   p.grad_type = grad_type;
   const int64_t items = most_items(s);
   NVTE_CHECK(items <= 65535, "too many work items: ", items);
@@ -1027,9 +1033,10 @@ void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const in
     NVTE_CHECK(w.bytes == 0 || aligned16(workspace), "the workspace must be 16-byte aligned");
     char *ws = static_cast<char *>(workspace);
     Plan plan{};
-    if (w.bytes != 0)
-      plan = prepare(s, adapter_ids, true, nullptr, nullptr, reinterpret_cast<int *>(ws + w.order),
-                     reinterpret_cast<int *>(ws + w.block_base), reinterpret_cast<int *>(ws + w.item_base), stream);
+    if (w.bytes != 0) {
+      plan = w.plan(ws);
+      prepare(s, adapter_ids, plan, true, nullptr, nullptr, stream);
+    }
     const ExpandArgs p{low, static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(base), scaling, adapter_ids, plan,
                        static_cast<uint16_t *>(out), s.tokens, num_slices(s.tokens, s.in), s.out, s.rank, s.num, 0};
     if (s.type == kNVTEBFloat16) {
