@@ -199,7 +199,7 @@ __device__ __forceinline__ float sum_slices(const float *p, int slices, int64_t 
 // ====================================================================================
 // expand: out[t][c] = base[t][c] + s_a sum_j (sum over slices of low[slice][t][j]) * w(c, j)
 // w(c, j) = pool[a][c][j], or pool[a][j][c] (RMAJOR)
-// Reads and writes 2 T O bytes each, which bounds it: 8192 x 14336, rank 32: 104 us (4.5 TB/s).  A decode tile is bound by its adapters
+// Reads and writes 2 T O bytes each, which bounds it: 8192 x 14336, rank 32: 100 us (4.7 TB/s; 106 with the old values asked for only once the rank vectors were there).  A decode tile is bound by its adapters
 // instead: 96 x 14336 with 48 of rank 16 (22 MB of pool, read about twice) 15 us.
 // ====================================================================================
 struct ExpandArgs {
@@ -262,8 +262,28 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   write |= todo;
   if (write == 0) return;
   const int begin = columns * p.cols, end = min(begin + p.cols, p.features);
-  // The pool's operands of the first step travel while the rank vectors are put together; later ones from the moment on that
-  // their predecessors are used up.
+  // All that the first step reads is on its way before anything waits: the rank vectors, which are needed first, then the pool's
+  // operands and the columns' old values; later ones from the moment on that their predecessors are used up.
+  const float scale = p.scaling != nullptr && id >= 0 ? p.scaling[id] : 1.f;
+  constexpr int kMine = 2 * MT * KT;  // values per thread
+  constexpr int kBatch = (MT == 1 ? 32 : 16) / kMine;  // slices on their way at once; many tokens have few
+  const float *low[kMine];
+#pragma unroll
+  for (int n = 0; n < kMine; ++n) {
+    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
+    low[n] = p.low + static_cast<int64_t>(__shfl(token, tok, 64)) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
+  }
+  const int64_t stride = p.tokens * p.rank;
+  float part[kBatch][kMine], v[kMine] = {};
+  auto load_low = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) part[i][n] = low[n][min(s0 + i, p.slices - 1) * stride];
+  };
+  load_low(0);
+  __builtin_amdgcn_sched_barrier(0);
+
   u32x4 f[KT][8];
   auto load_pool = [&](uint64_t left, int c0) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
@@ -273,59 +293,17 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   int c0 = begin + wave * 128;
   if (todo != 0 && c0 < end) load_pool(todo, c0);
 
-  const float scale = p.scaling != nullptr && id >= 0 ? p.scaling[id] : 1.f;
-  constexpr int kMine = 2 * MT * KT;  // values per thread
-  float v[kMine] = {};
-  const float *low[kMine];
-#pragma unroll
-  for (int n = 0; n < kMine; ++n) {
-    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
-    low[n] = p.low + static_cast<int64_t>(__shfl(token, tok, 64)) * p.rank + max(slot_rank(j, p.rank, RMAJOR), 0);
-  }
-  const int64_t stride = p.tokens * p.rank;
-  constexpr int kBatch = 32 / kMine;  // loads on their way at once
-  for (int s0 = 0; s0 < p.slices; s0 += kBatch) {
-    float part[kBatch][kMine];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-      for (int n = 0; n < kMine; ++n) part[i][n] = low[n][min(s0 + i, p.slices - 1) * stride];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-      for (int n = 0; n < kMine; ++n) v[n] += s0 + i < p.slices ? part[i][n] : 0.f;
-  }
-#pragma unroll
-  for (int n = 0; n < kMine; ++n) {
-    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
-    const float s = __shfl(scale, tok, 64);
-    __bf16 h, l;
-    split1(((todo >> tok) & 1) && slot_rank(j, p.rank, RMAJOR) >= 0 ? s * v[n] : 0.f, h, l);
-    s_hi[tok][j] = bits16(h);
-    s_lo[tok][j] = bits16(l);
-  }
-  // only the LDS writes have to be done: the pool's loads stay on their way
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  u32x4 hi[MT][KT], lo[MT][KT];
   int my_id[MT][4];       // of the lane's four tokens per subtile
   int row[MT][4];         // they themselves; one that is not written here reads the first that is
   const int any = __builtin_ctzll(write);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int tok = m * 16 + 4 * (lane >> 4) + i;
       my_id[m][i] = __shfl(id, tok, 64);
       row[m][i] = __shfl(token, ((write >> tok) & 1) ? tok : any, 64);
     }
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      hi[m][k] = *reinterpret_cast<const u32x4 *>(&s_hi[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
-      lo[m][k] = *reinterpret_cast<const u32x4 *>(&s_lo[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
-    }
-  }
   // the columns' old values travel a step ahead
   u32x4 base[MT][4], ahead[MT][4];
   auto load_base = [&](int c0, u32x4 (&v)[MT][4]) {
@@ -346,6 +324,37 @@ __device__ __forceinline__ void expand_tile(const ExpandArgs &p, int64_t tile, i
   } else if (c0 < end) {
     load_base(c0, base);
   }
+  __builtin_amdgcn_sched_barrier(0);
+
+  for (int s0 = 0;;) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) v[n] += s0 + i < p.slices ? part[i][n] : 0.f;
+    if ((s0 += kBatch) >= p.slices) break;
+    load_low(s0);
+  }
+#pragma unroll
+  for (int n = 0; n < kMine; ++n) {
+    const int e = threadIdx.x + 256 * n, tok = e / (KT * 32), j = e % (KT * 32);
+    const float s = __shfl(scale, tok, 64);
+    __bf16 h, l;
+    split1(((todo >> tok) & 1) && slot_rank(j, p.rank, RMAJOR) >= 0 ? s * v[n] : 0.f, h, l);
+    s_hi[tok][j] = bits16(h);
+    s_lo[tok][j] = bits16(l);
+  }
+  // only the LDS writes have to be done: the loads stay on their way
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  u32x4 hi[MT][KT], lo[MT][KT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      hi[m][k] = *reinterpret_cast<const u32x4 *>(&s_hi[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
+      lo[m][k] = *reinterpret_cast<const u32x4 *>(&s_lo[m * 16 + (lane & 15)][k * 32 + (lane >> 4) * 8]);
+    }
   f32x4 res[MT][8];
   uint64_t left = todo;
   while (c0 < end) {
