@@ -94,6 +94,8 @@ SHAPES = [  # tokens, in, out, rank, adapters
     (1100, 7, 5, 66, 3),
     (4500, 264, 512, 24, 3),
     (4100, 136, 72, 64, 1),
+    (4096, 40, 24, 8, 70),
+    (8200, 24, 40, 8, 4096),
 ]
 
 
