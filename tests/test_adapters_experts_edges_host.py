@@ -1,0 +1,50 @@
+"""Refusals at the edges of the adapter, expert and clipping entry points that need no GPU (addresses are made up and never read)."""
+import ctypes as C
+
+import pytest
+
+from transformer_engine_amd import NVTEError
+from transformer_engine_amd._lib import api, kFloat32
+
+P = 0x1000
+
+
+def _list(**k):
+    d = dict(grads=(C.c_void_p * 1)(P), outs=(C.c_void_p * 1)(2 * P), numels=(C.c_size_t * 1)(4), dtypes=(C.c_int * 1)(kFloat32),
+             out_dtypes=(C.c_int * 1)(kFloat32))
+    d.update(k)
+    return list(d.values()) + [1]
+
+
+def clip(ws=P, size=1 << 20, norm=0, **k):
+    api.nvte_amd_clip_grad_norm(*_list(**k), C.c_float(1.0), C.c_float(1e-6), norm, ws, size, 0)
+
+
+def clip_by_sum(sum_of_squares=P, norm=0, **k):
+    api.nvte_amd_clip_by_sum_of_squares(*_list(**k), sum_of_squares, C.c_float(1.0), C.c_float(1e-6), norm, 0)
+
+
+def grad_norm(ws=P, size=1 << 20, total=0, norm=0, **k):
+    grads, _, numels, dtypes, _, n = _list(**k)
+    api.nvte_amd_grad_norm(grads, numels, dtypes, n, total, norm, ws, size, 0)
+
+
+@pytest.mark.parametrize("missing", ["grads", "outs", "numels", "dtypes", "out_dtypes"])
+@pytest.mark.parametrize("call", [clip, clip_by_sum])
+def test_clipping_refuses_missing_lists(call, missing):
+    with pytest.raises(NVTEError, match="NULL"):
+        call(**{missing: 0})
+
+
+@pytest.mark.parametrize("missing", ["grads", "numels", "dtypes"])
+def test_norm_refuses_missing_lists(missing):
+    with pytest.raises(NVTEError, match="NULL"):
+        grad_norm(**{missing: 0})
+
+
+@pytest.mark.parametrize("call, bad", [(clip, dict(ws=P + 4)), (grad_norm, dict(ws=P + 4)), (clip_by_sum, dict(sum_of_squares=P + 4)),
+                                       (grad_norm, dict(total=P + 4)), (clip, dict(norm=P + 2)), (grad_norm, dict(norm=P + 2)),
+                                       (clip_by_sum, dict(norm=P + 2))])
+def test_clipping_refuses_misaligned_sums(call, bad):
+    with pytest.raises(NVTEError, match="aligned"):
+        call(**bad)

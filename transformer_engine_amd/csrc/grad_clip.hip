@@ -227,8 +227,9 @@ int64_t num_chunks(const size_t *numel, size_t n, int64_t chunk) {
   return c;
 }
 
-void check_list(const List &l) {
-  NVTE_CHECK(l.n == 0 || (l.in && l.numel && l.in_type), "null tensor list");
+void check_list(const List &l, bool clips) {
+  NVTE_CHECK(l.n == 0 || (l.in && l.numel && l.in_type), "a list of the gradients is NULL");
+  NVTE_CHECK(l.n == 0 || !clips || (l.out && l.out_type), "outs or out_dtypes is NULL");
   for (size_t i = 0; i < l.n; ++i) {
     NVTE_CHECK(is_high_precision(static_cast<DType>(l.in_type[i])), "gradient ", i, " has dtype=",
                dtype_name(static_cast<DType>(l.in_type[i])), ", but expected float32, float16 or bfloat16");
@@ -327,6 +328,10 @@ void clip(const List &l, int64_t chunk, const double *slots, int64_t num_slots, 
   if (!any && norm != nullptr) add_slots(slots, num_slots, nullptr, norm, stream);  // nothing but empty tensors
 }
 
+void check_aligned(const char *what, const void *p, size_t align) {
+  NVTE_CHECK(reinterpret_cast<uintptr_t>(p) % align == 0, what, " must be ", align, "-byte aligned");
+}
+
 void check_clip(float max_norm, float eps) {
   NVTE_CHECK(max_norm >= 0.f, "max_norm must not be negative or NaN, got ", max_norm);
   NVTE_CHECK(eps >= 0.f && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
@@ -350,7 +355,10 @@ void nvte_amd_grad_norm(const void *const *grads, const size_t *numels, const in
                         double *sum_of_squares, float *norm, void *workspace, size_t workspace_bytes, hipStream_t stream) {
   api_guard("nvte_amd_grad_norm", [&] {
     const List l{grads, nullptr, numels, dtypes, nullptr, num_tensors};
-    check_list(l);
+    check_list(l, false);
+    check_aligned("the workspace", workspace, sizeof(double));
+    check_aligned("sum_of_squares", sum_of_squares, sizeof(double));
+    check_aligned("norm", norm, sizeof(float));
     const int64_t chunk = chunk_size_of(numels, num_tensors), slots = num_chunks(numels, num_tensors, chunk);
     NVTE_CHECK(workspace != nullptr && workspace_bytes >= static_cast<size_t>(slots + 1) * sizeof(double),
                "workspace of ", workspace_bytes, " bytes, but ", (slots + 1) * sizeof(double), " are needed");
@@ -365,9 +373,10 @@ void nvte_amd_clip_grad_norm(const void *const *grads, void *const *outs, const 
                              void *workspace, size_t workspace_bytes, hipStream_t stream) {
   api_guard("nvte_amd_clip_grad_norm", [&] {
     const List l{grads, outs, numels, dtypes, out_dtypes, num_tensors};
-    check_list(l);
-    NVTE_CHECK(num_tensors == 0 || (outs != nullptr && out_dtypes != nullptr), "outs is NULL");
+    check_list(l, true);
     check_clip(max_norm, eps);
+    check_aligned("the workspace", workspace, sizeof(double));
+    check_aligned("norm", norm, sizeof(float));
     const int64_t chunk = chunk_size_of(numels, num_tensors), slots = num_chunks(numels, num_tensors, chunk);
     NVTE_CHECK(workspace != nullptr && workspace_bytes >= static_cast<size_t>(slots + 1) * sizeof(double),
                "workspace of ", workspace_bytes, " bytes, but ", (slots + 1) * sizeof(double), " are needed");
@@ -387,10 +396,11 @@ void nvte_amd_clip_by_sum_of_squares(const void *const *grads, void *const *outs
                                      float eps, float *norm, hipStream_t stream) {
   api_guard("nvte_amd_clip_by_sum_of_squares", [&] {
     const List l{grads, outs, numels, dtypes, out_dtypes, num_tensors};
-    check_list(l);
-    NVTE_CHECK(num_tensors == 0 || (outs != nullptr && out_dtypes != nullptr), "outs is NULL");
+    check_list(l, true);
     NVTE_CHECK(sum_of_squares != nullptr, "sum_of_squares is NULL");
     check_clip(max_norm, eps);
+    check_aligned("sum_of_squares", sum_of_squares, sizeof(double));
+    check_aligned("norm", norm, sizeof(float));
     clip(l, chunk_size_of(numels, num_tensors), sum_of_squares, 1, max_norm, eps, norm, stream);
   });
 }
