@@ -121,9 +121,11 @@ void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const in
                            hipStream_t stream);
 /* dx[t] = base_grad[t] + scaling[id] a[id]^T (b[id]^T dy[t]); da [num_adapters, rank, in] and db [num_adapters, out, rank], in
  * dtype or fp32 (grad_dtype), are sums over each adapter's tokens in a fixed order, zero for an adapter without tokens.  dx may
- * be NULL, da and db may be NULL together; base_grad NULL = zero, or dx itself.  Up to 4096 adapters when da / db are wanted. */
+ * be NULL, da and db may be NULL together; base_grad NULL = zero, or dx itself.  Up to 4096 adapters when da / db are wanted.
+ * The first size is that of a call with da and db, the second (a part of it) that of a call without them. */
 size_t nvte_amd_lora_backward_workspace_size(size_t tokens, size_t in_features, size_t out_features, size_t rank,
                                              size_t num_adapters);
+size_t nvte_amd_lora_dgrad_workspace_size(size_t tokens, size_t out_features, size_t rank, size_t num_adapters);
 void nvte_amd_lora_backward(const void *x, const void *dy, const void *a, const void *b, const int *adapter_ids,
                             const float *scaling, const float *low, const void *base_grad, void *dx, void *da, void *db,
                             size_t tokens, size_t in_features, size_t out_features, size_t rank, size_t num_adapters,

@@ -1,0 +1,44 @@
+"""Adapters, experts and clipping at the edges of what their entry points allow: memory, gradients that must not get lost, calls at
+once, the largest sizes."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import test_lora_gpu as lora_tests
+    from transformer_engine_amd._lib import api, kBFloat16
+    from transformer_engine_amd.lora import lora_backward, lora_forward
+    from transformer_engine_amd.tensor import current_stream_ptr
+
+
+@pytest.mark.parametrize("t, n", [(3, 5), (40, 300), (700, 6), (700, 1), (520, 5000)])
+def test_activation_gradients_alone_stay_in_their_own_workspace(t, n):
+    k, o, r = 136, 264, 24
+    x, a, b, ids, s, _, dy, gbase = lora_tests.make(t, k, o, r, n, torch.bfloat16, seed=t + n)
+    want = lora_tests.oracle(x, a, b, ids, s, None, dy, gbase)
+    size = api.nvte_amd_lora_dgrad_workspace_size(t, o, r, n)
+    ws = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    dx = torch.empty_like(x)
+    api.nvte_amd_lora_backward(x.data_ptr(), dy.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), s.data_ptr(), x.data_ptr(),
+                               gbase.data_ptr(), dx.data_ptr(), 0, 0, t, k, o, r, n, kBFloat16, kBFloat16, ws.data_ptr(), size,
+                               current_stream_ptr())     # `low` is not read without weight gradients
+    assert (ws[size:] == 0xA5).all()
+    lora_tests.check("dx", dx, want[0]["dx"], want[1]["dx"], o + r + 2)
+    _, saved = lora_forward(x, a, b, ids, s)
+    assert torch.equal(lora_backward(dy, saved, base_grad=gbase, requires_wgrad=False)[0], dx)
+    if n <= 4096:
+        assert torch.equal(lora_backward(dy, saved, base_grad=gbase)[0], dx)
+
+
+def test_activation_gradients_alone_take_little_memory():
+    t, k, o, r, n = 64, 2048, 4096, 16, 512
+    x, a, b, ids, s, _, dy, _ = lora_tests.make(t, k, o, r, n, torch.bfloat16, std=0.1)
+    _, saved = lora_forward(x, a, b, ids, s)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    lora_backward(dy, saved, requires_wgrad=False)
+    taken = torch.cuda.max_memory_allocated() - before
+    # B transposed, partial rank vectors and dx; weight gradients' partial sums alone would be 64 * 16 * (2048 + 4096) * 4 = 25 MB
+    assert taken <= b.numel() * 2 + 2 * t * k + 64 * t * r * 4 + (2 << 20), taken

@@ -48,3 +48,29 @@ def test_norm_refuses_missing_lists(missing):
 def test_clipping_refuses_misaligned_sums(call, bad):
     with pytest.raises(NVTEError, match="aligned"):
         call(**bad)
+
+
+@pytest.mark.parametrize("tokens, k, o, rank, n", [(4096, 4096, 14336, 64, 4096), (8, 4096, 14336, 16, 512), (600, 64, 96, 128, 7),
+                                                   (64, 2056, 2731, 20, 9000), (8192, 4096, 4096, 16, 1)])
+def test_a_pass_without_weight_gradients_needs_no_space_for_them(tokens, k, o, rank, n):
+    size = api.nvte_amd_lora_dgrad_workspace_size(tokens, o, rank, n)
+    rank_vectors = api.nvte_amd_lora_num_slices(tokens, o) * tokens * rank * 4
+    lists = (tokens + 32 * (n + 1)) * 5 + 1024       # every adapter's tokens in blocks of 32, and each block's adapter
+    assert 0 < size <= rank_vectors + n * rank * o * 2 + lists + 5 * 256
+    if n <= 4096:
+        assert size < api.nvte_amd_lora_backward_workspace_size(tokens, k, o, rank, n)
+
+
+def _backward(ws, size, da=P, db=P, tokens=8, n=512):
+    api.nvte_amd_lora_backward(P, P, P, P, P, 0, P, 0, P, da, db, tokens, 4096, 14336, 16, n, 6, 6, ws, size, 0)
+
+
+def test_workspace_of_a_pass_without_weight_gradients_is_checked_by_its_own_size():
+    small, large = api.nvte_amd_lora_dgrad_workspace_size(8, 14336, 16, 512), \
+        api.nvte_amd_lora_backward_workspace_size(8, 4096, 14336, 16, 512)
+    for bad in (dict(ws=P, size=small - 1, da=0, db=0), dict(ws=0, size=small, da=0, db=0), dict(ws=P, size=small),
+                dict(ws=P, size=large - 1)):
+        with pytest.raises(NVTEError, match="workspace of"):
+            _backward(**bad)
+    assert api.nvte_amd_lora_dgrad_workspace_size(0, 14336, 16, 512) == 0
+    _backward(0, 0, da=0, db=0, tokens=0)               # nothing to do, nothing launched

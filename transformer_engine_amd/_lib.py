@@ -124,6 +124,7 @@ _SIGS = {
     "nvte_amd_lora_forward_workspace_size": (_SZ, [_SZ, _SZ]),
     "nvte_amd_lora_forward": (_V, [_P] * 8 + [_SZ] * 5 + [_I, _P, _SZ, _P]),
     "nvte_amd_lora_backward_workspace_size": (_SZ, [_SZ] * 5),
+    "nvte_amd_lora_dgrad_workspace_size": (_SZ, [_SZ] * 4),
     "nvte_amd_lora_backward": (_V, [_P] * 11 + [_SZ] * 5 + [_I, _I, _P, _SZ, _P]),
     "nvte_amd_moe_topk": (_V, [_P, _P, _P, _SZ, _SZ, _SZ, _I, _I, _P]),
     "nvte_amd_moe_forward_workspace_size": (_SZ, [_SZ] * 5),

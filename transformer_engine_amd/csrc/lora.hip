@@ -797,7 +797,7 @@ int phases_of(int64_t workgroups, int64_t tokens, int num) {
 }
 
 // every list's last block may be partly filled
-int64_t most_blocks(int64_t tokens, int num) { return tokens / kBlock + std::min<int64_t>(num + 1, tokens); }
+int64_t most_blocks(int64_t tokens, int num) { return tokens / kBlock + std::min<int64_t>(num + 1ll, tokens); }
 int64_t tiles_of(const Plan &plan, int64_t tokens, int num, int size) {
   return plan.order != nullptr ? most_blocks(tokens, num) * kBlock / size : static_cast<int64_t>(ceil_div(tokens, size));
 }
@@ -945,20 +945,30 @@ ForwardWorkspace forward_workspace(int64_t tokens, int num) {
 
 struct BackwardWorkspace {
   size_t low, transposed, order, owner, ends, item_base, items, packed_a, packed_b, part_a, part_b, bytes;
+  bool lists, wgrad;
   Plan plan(char *ws) const {
+    if (!lists) return {};
     return {reinterpret_cast<int *>(ws + order), reinterpret_cast<int *>(ws + owner), reinterpret_cast<int *>(ws + ends),
-            reinterpret_cast<int *>(ws + item_base), reinterpret_cast<int2 *>(ws + items)};
+            wgrad ? reinterpret_cast<int *>(ws + item_base) : nullptr, wgrad ? reinterpret_cast<int2 *>(ws + items) : nullptr};
   }
 };
-BackwardWorkspace backward_workspace(const Shape &s) {
+// Weight gradients take by far the most of it (a share of [rank][in + out] in fp32 for every work item), so a pass without them
+// has a size of its own, in which `in` has no part.
+BackwardWorkspace backward_workspace(const Shape &s, bool wgrad) {
   BackwardWorkspace w{};
   Space space;
   auto take = [&](size_t bytes) { return space.take(bytes); };
+  w.wgrad = wgrad;
+  w.lists = wgrad || ordered(s.tokens, s.num);
   w.low = take(static_cast<size_t>(num_slices(s.tokens, s.out)) * s.tokens * s.rank * sizeof(float));
-  w.transposed = take(static_cast<size_t>(s.num) * s.rank * s.out * 2);
-  w.order = take(most_blocks(s.tokens, s.num) * kBlock * sizeof(int));
-  w.owner = take(most_blocks(s.tokens, s.num) * sizeof(int));
-  w.ends = take(2 * sizeof(int));
+  w.transposed = take(s.tokens > 0 ? static_cast<size_t>(s.num) * s.rank * s.out * 2 : 0);
+  if (w.lists) {
+    w.order = take(most_blocks(s.tokens, s.num) * kBlock * sizeof(int));
+    w.owner = take(most_blocks(s.tokens, s.num) * sizeof(int));
+    w.ends = take(2 * sizeof(int));
+  }
+  w.bytes = space.at;
+  if (!wgrad) return w;
   w.item_base = take((static_cast<size_t>(s.num) + 1) * sizeof(int));
   w.items = take(most_items(s) * sizeof(int2));
   const size_t packed = static_cast<size_t>(most_blocks(s.tokens, s.num)) * ceil_div(s.rank, 16) * 2048;
@@ -973,13 +983,13 @@ BackwardWorkspace backward_workspace(const Shape &s) {
 template <typename E>
 void backward(const Shape &s, const void *x, const void *dy, const void *a, const void *b, const int *ids, const float *scaling,
               const float *low, const void *base_grad, void *dx, void *da, void *db, int grad_type, char *ws, hipStream_t stream) {
-  const BackwardWorkspace w = backward_workspace(s);
-  float *up = reinterpret_cast<float *>(ws + w.low);
-  uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
   const bool wgrad = da != nullptr, in_order = ordered(s.tokens, s.num);
   if (!wgrad && (dx == nullptr || s.tokens == 0)) return;
+  const BackwardWorkspace w = backward_workspace(s, wgrad);
+  float *up = reinterpret_cast<float *>(ws + w.low);
+  uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
   const Plan plan = w.plan(ws);
-  prepare(s, ids, plan, wgrad || in_order, s.tokens > 0 ? b : nullptr, bt, stream);
+  prepare(s, ids, plan, w.lists, s.tokens > 0 ? b : nullptr, bt, stream);
   const Plan tiles = in_order ? plan : Plan{};
   const int64_t blocks = wgrad ? most_blocks(s.tokens, s.num) : 0;
   uint16_t *packed_a = reinterpret_cast<uint16_t *>(ws + w.packed_a), *packed_b = reinterpret_cast<uint16_t *>(ws + w.packed_b);
@@ -1064,7 +1074,13 @@ void nvte_amd_lora_forward(const void *x, const void *a, const void *b, const in
 size_t nvte_amd_lora_backward_workspace_size(size_t tokens, size_t in_features, size_t out_features, size_t rank,
                                              size_t num_adapters) {
   return api_guard("nvte_amd_lora_backward_workspace_size", [&]() -> size_t {
-    return backward_workspace(shape_of(tokens, in_features, out_features, rank, num_adapters, kNVTEBFloat16)).bytes;
+    return backward_workspace(shape_of(tokens, in_features, out_features, rank, num_adapters, kNVTEBFloat16), true).bytes;
+  });
+}
+
+size_t nvte_amd_lora_dgrad_workspace_size(size_t tokens, size_t out_features, size_t rank, size_t num_adapters) {
+  return api_guard("nvte_amd_lora_dgrad_workspace_size", [&]() -> size_t {
+    return backward_workspace(shape_of(tokens, 1, out_features, rank, num_adapters, kNVTEBFloat16), false).bytes;
   });
 }
 
@@ -1079,8 +1095,8 @@ void nvte_amd_lora_backward(const void *x, const void *dy, const void *a, const 
     NVTE_CHECK((da == nullptr) == (db == nullptr), "da and db come together");
     NVTE_CHECK(da == nullptr || s.num <= kMaxAdapters, "a backward pass takes up to ", kMaxAdapters, " adapters, got ", s.num);
     NVTE_CHECK(s.tokens == 0 || (x && dy && a && b && adapter_ids && low), "a required pointer is NULL");
-    const size_t need = backward_workspace(s).bytes;
-    NVTE_CHECK(workspace != nullptr && workspace_bytes >= need, "workspace of ", workspace_bytes, " bytes, but ", need, " are needed");
+    const size_t need = backward_workspace(s, da != nullptr).bytes;
+    NVTE_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace of ", workspace_bytes, " bytes, but ", need, " are needed");
     NVTE_CHECK(aligned16(workspace), "the workspace must be 16-byte aligned");
     char *ws = static_cast<char *>(workspace);
     if (s.type == kNVTEBFloat16)

@@ -150,7 +150,8 @@ def lora_backward(dy: torch.Tensor, saved: LoRASaved, base_grad: Optional[torch.
     dx = torch.empty(x_shape, dtype=x.dtype, device=dev) if requires_dgrad else None
     da = torch.empty(a.shape, dtype=gdt, device=dev) if requires_wgrad else None
     db = torch.empty(b.shape, dtype=gdt, device=dev) if requires_wgrad else None
-    size = api.nvte_amd_lora_backward_workspace_size(tokens, k, o, rank, n)
+    size = (api.nvte_amd_lora_backward_workspace_size(tokens, k, o, rank, n) if requires_wgrad
+            else api.nvte_amd_lora_dgrad_workspace_size(tokens, o, rank, n))
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     ptr = lambda t: 0 if t is None else t.data_ptr()
     api.nvte_amd_lora_backward(x.data_ptr(), dy.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), ptr(scaling),
