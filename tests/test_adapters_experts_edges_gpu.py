@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     import test_lora_gpu as lora_tests
     from transformer_engine_amd._lib import api, kBFloat16
-    from transformer_engine_amd.lora import lora_backward, lora_forward
+    from transformer_engine_amd.lora import LoRALinear, lora, lora_backward, lora_forward
     from transformer_engine_amd.tensor import current_stream_ptr
 
 
@@ -42,3 +42,42 @@ def test_activation_gradients_alone_take_little_memory():
     taken = torch.cuda.max_memory_allocated() - before
     # B transposed, partial rank vectors and dx; weight gradients' partial sums alone would be 64 * 16 * (2048 + 4096) * 4 = 25 MB
     assert taken <= b.numel() * 2 + 2 * t * k + 64 * t * r * 4 + (2 << 20), taken
+
+
+def _penalty(f, at):
+    """f and the sum of its gradient's squares, as a gradient penalty adds them."""
+    y = f()
+    g, = torch.autograd.grad(y.float().sum(), (at,), create_graph=True)
+    return y.float().sum() + g.float().square().sum()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_second_derivatives_of_adapters_raise(which):
+    x, a, b, ids, s, base, _, _ = lora_tests.make(20, 64, 96, 8, 3, torch.bfloat16)
+    args = [v.requires_grad_() for v in (x, a, b)]
+    loss = _penalty(lambda: lora(*args, ids, s, base), args[which])
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        loss.backward()
+
+
+def test_first_derivatives_and_the_projections_own_chain_go_on():
+    x, a, b, ids, s, base, dy, _ = lora_tests.make(20, 64, 96, 8, 3, torch.bfloat16)
+    x, a, b, base = (v.requires_grad_() for v in (x, a, b, base))
+    lora(x, a, b, ids, s, base).backward(dy)
+    assert not any(v.grad.requires_grad for v in (x, a, b, base))
+    want = [v.grad.clone() for v in (x, a, b, base)]
+    got = torch.autograd.grad(lora(x, a, b, ids, s, base), (x, a, b, base), dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    scale = torch.ones((), device="cuda", dtype=torch.bfloat16, requires_grad=True)   # dy reaches base unchanged, any number of times
+    g, = torch.autograd.grad(lora(x, a, b, ids, s, base), (base,), dy * scale, create_graph=True)
+    g.float().sum().backward(inputs=[scale])
+    want = dy.float().sum()
+    assert abs(scale.grad.float() - want) <= 2.0 ** -8 * dy.float().abs().sum()   # dy * scale, its gradient's sum and result in bf16
+
+
+def test_second_derivatives_of_the_module_raise():
+    m = LoRALinear(64, 96, rank=8)
+    x = torch.randn(32, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    for at in (x, m.lora_a, m.lora_b):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            _penalty(lambda: m(x), at).backward()

@@ -23,7 +23,7 @@ import torch
 
 from ._lib import api
 from .linear import Linear, linear_backward, linear_forward
-from .tensor import current_stream_ptr, te_dtype
+from .tensor import current_stream_ptr, refuse_gradient, te_dtype
 
 __all__ = ["lora_forward", "lora_backward", "lora", "LoRALinear"]
 
@@ -169,6 +169,11 @@ def _load(ctx) -> LoRASaved:
     return LoRASaved(*ctx.saved_tensors, ctx.x_shape)
 
 
+def _first_order(*grads):
+    """What a backward pass returns: under ``create_graph`` gradients that raise when they are differentiated themselves."""
+    return refuse_gradient("adapters have no second derivatives", *grads) if torch.is_grad_enabled() else grads
+
+
 class _LoRAFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, adapter_ids, scaling, base):
@@ -179,13 +184,13 @@ class _LoRAFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        dx, da, db = lora_backward(dy, _load(ctx), requires_dgrad=need[0], requires_wgrad=need[1] or need[2])
+        dx, da, db = _first_order(*lora_backward(dy, _load(ctx), requires_dgrad=need[0], requires_wgrad=need[1] or need[2]))
         return dx, da, db, None, None, dy if need[5] else None
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
          scaling: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``base + scaling * B (A x)``, differentiable in x, a, b and base (``scaling`` is a constant)."""
+    """``base + scaling * B (A x)``, differentiable once in x, a, b and base (``scaling`` is a constant)."""
     return _LoRAFn.apply(x, a, b, adapter_ids, scaling, base)
 
 
@@ -209,8 +214,8 @@ class _LoRALinearFn(torch.autograd.Function):
             base_grad, _, _ = linear_backward(dy, ctx.saved_q, lin.fp8_state, requires_wgrad=False)
             base_grad = base_grad.reshape(ctx.x_shape)
             lin.fp8_state.update_bwd(lin.amax_group)
-        dx, da, db = lora_backward(dy, _load(ctx), base_grad=base_grad, requires_dgrad=need[0],
-                                   requires_wgrad=need[1] or need[2])
+        dx, da, db = _first_order(*lora_backward(dy, _load(ctx), base_grad=base_grad, requires_dgrad=need[0],
+                                                 requires_wgrad=need[1] or need[2]))
         return dx, da, db, None, None, None
 
 

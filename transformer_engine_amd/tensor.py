@@ -76,6 +76,24 @@ def current_stream_ptr() -> int:
     return int(torch.cuda.current_stream().cuda_stream)
 
 
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, message, anchor, *values):
+        ctx.message = message
+        return values
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(ctx.message)
+
+
+def refuse_gradient(message: str, *values: Optional[torch.Tensor]):
+    """``values`` (None among them) as results through which no gradient flows: differentiating them raises ``message``, where plain
+    kernel results would drop their share of the sum without a word."""
+    done = iter(_NoGradient.apply(message, torch.empty(0, requires_grad=True), *(v for v in values if v is not None)))
+    return tuple(None if v is None else next(done) for v in values)
+
+
 def non_tn_fp8_gemm_supported() -> bool:
     return bool(api.nvte_is_non_tn_fp8_gemm_supported())
 
