@@ -81,3 +81,17 @@ def test_second_derivatives_of_the_module_raise():
     for at in (x, m.lora_a, m.lora_b):
         with pytest.raises(RuntimeError, match="second derivatives"):
             _penalty(lambda: m(x), at).backward()
+
+
+def test_a_projection_that_is_trained_is_refused():
+    m = LoRALinear(64, 96, rank=8)
+    x = torch.randn(32, 64, device="cuda", dtype=torch.bfloat16)
+    for p in (m.linear.weight, m.linear.bias):
+        p.requires_grad_()
+        with pytest.raises(RuntimeError, match="frozen"):
+            m(x)
+        with torch.no_grad():
+            assert torch.isfinite(m(x).float()).all()
+        p.requires_grad_(False)
+    m(x).float().sum().backward()
+    assert m.lora_b.grad is not None

@@ -224,7 +224,8 @@ class LoRALinear(torch.nn.Module):
 
     ``lora_a`` [num_adapters, rank, in] starts random and ``lora_b`` [num_adapters, out, rank] at zero, so a new adapter changes
     nothing; ``scaling`` is ``alpha / rank`` for every adapter (``alpha`` defaults to the rank).  Without ``adapter_ids`` every token
-    uses adapter 0.  ``is_first_microbatch`` keeps the shared weight's FP8 copy over calls as ``Linear`` does."""
+    uses adapter 0.  A projection whose parameters require a gradient is refused: it would get none (``Linear`` and ``lora`` train
+    both).  ``is_first_microbatch`` keeps the shared weight's FP8 copy over calls as ``Linear`` does."""
 
     def __init__(self, in_features: int, out_features: int, rank: int, num_adapters: int = 1, alpha: Optional[float] = None,
                  bias: bool = True, params_dtype: torch.dtype = torch.bfloat16, device="cuda", recipe=None):
@@ -246,6 +247,9 @@ class LoRALinear(torch.nn.Module):
         if adapter_ids is None:
             adapter_ids = torch.zeros(x.shape[:-1], dtype=torch.int32, device=x.device)
         _check(x, self.lora_a, self.lora_b, adapter_ids, self.scaling)
+        if torch.is_grad_enabled() and any(p.requires_grad for p in self.linear.parameters()):
+            raise RuntimeError("the projection of a LoRALinear is frozen, but its weight or bias requires a gradient: call "
+                               "requires_grad_(False) on it, or use Linear and lora to train both")
         self._is_first_microbatch = is_first_microbatch
         self._needs_backward = torch.is_grad_enabled()
         y = _LoRALinearFn.apply(x, self.lora_a, self.lora_b, adapter_ids, self.scaling, self)
