@@ -95,3 +95,12 @@ def test_a_projection_that_is_trained_is_refused():
         p.requires_grad_(False)
     m(x).float().sum().backward()
     assert m.lora_b.grad is not None
+
+
+def test_a_scaling_that_is_trained_is_refused():
+    x, a, b, ids, s, base, _, _ = lora_tests.make(20, 64, 96, 8, 3, torch.bfloat16)
+    s.requires_grad_()
+    with pytest.raises(RuntimeError, match="scaling"):
+        lora(x, a, b, ids, s, base)
+    with torch.no_grad():
+        lora(x, a, b, ids, s, base)

@@ -191,6 +191,8 @@ class _LoRAFn(torch.autograd.Function):
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
          scaling: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``base + scaling * B (A x)``, differentiable once in x, a, b and base (``scaling`` is a constant)."""
+    if scaling is not None and scaling.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("scaling is a constant of the adapters and gets no gradient: detach it")
     return _LoRAFn.apply(x, a, b, adapter_ids, scaling, base)
 
 
