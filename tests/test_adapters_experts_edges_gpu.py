@@ -7,8 +7,10 @@ pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
     import test_lora_gpu as lora_tests
+    import test_moe_gpu as moe_tests
     from transformer_engine_amd._lib import api, kBFloat16
     from transformer_engine_amd.lora import LoRALinear, lora, lora_backward, lora_forward
+    from transformer_engine_amd.moe import moe_forward, moe_topk
     from transformer_engine_amd.tensor import current_stream_ptr
 
 
@@ -104,3 +106,24 @@ def test_a_scaling_that_is_trained_is_refused():
         lora(x, a, b, ids, s, base)
     with torch.no_grad():
         lora(x, a, b, ids, s, base)
+
+
+def test_expert_layers_do_not_lose_gradients():
+    x, w1, w2, ids, weights, _, _ = moe_tests.make(5, 64, 48, 4, 2, torch.bfloat16)
+    plain = moe_forward(x, w1, w2, ids, weights)
+    assert not plain.requires_grad
+    for i in (0, 1, 2, 4):
+        args = [v.clone() for v in (x, w1, w2, ids, weights)]
+        args[i].requires_grad_()
+        out = moe_forward(*args)
+        assert torch.equal(out, plain)
+        with pytest.raises(RuntimeError, match="GroupedLinear"):
+            out.float().sum().backward()
+        with torch.no_grad():
+            assert not moe_forward(*args).requires_grad
+    logits = torch.randn(5, 4, device="cuda")
+    want = moe_topk(logits, 2)
+    top, w = moe_topk(logits.clone().requires_grad_(), 2)
+    assert torch.equal(top, want[0]) and torch.equal(w, want[1]) and not top.requires_grad
+    with pytest.raises(RuntimeError, match="moe_topk"):
+        w.sum().backward()

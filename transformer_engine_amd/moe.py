@@ -5,7 +5,8 @@
 
 The experts' weights are read once per batch and the routing stays on the device, as in ``grouped``: nothing is sorted or padded on
 the host, and the three launches of ``moe_forward`` can be captured into a HIP graph.  Batches of more than 256 tokens and training
-are ``grouped_linear``'s: there is no backward pass here, results carry no gradient.  The gate order is that of
+are ``grouped_linear``'s: there is no backward pass here, and a result of inputs that require a gradient raises when it is
+differentiated.  The gate order is that of
 ``activation("swiglu", ...)``: activation half first.
 """
 from __future__ import annotations
@@ -17,7 +18,7 @@ import torch
 from . import _lib
 from ._lib import api
 from .grouped import GroupedTensor
-from .tensor import DType, current_stream_ptr, te_dtype
+from .tensor import DType, current_stream_ptr, refuse_gradient, te_dtype
 
 __all__ = ["moe_topk", "moe_forward"]
 
@@ -45,6 +46,8 @@ def moe_topk(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Tupl
     weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
     api.nvte_amd_moe_topk(logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), tokens, experts, top_k, int(bool(renormalize)),
                           int(te_dtype(logits.dtype)), current_stream_ptr())
+    if logits.requires_grad and torch.is_grad_enabled():
+        weights, = refuse_gradient("moe_topk has no backward pass", weights)
     return ids, weights
 
 
@@ -120,4 +123,6 @@ def moe_forward(x: torch.Tensor, w_fc1: Union[torch.Tensor, GroupedTensor], w_fc
     api.nvte_amd_moe_forward(x2d.data_ptr(), w1.data_ptr(), w2.data_ptr(), s1.data_ptr() if fp8 else 0,
                              s2.data_ptr() if fp8 else 0, ids.data_ptr(), weights.data_ptr(), out.data_ptr(), tokens, top_k,
                              experts, hidden, ffn, int(te_dtype(x.dtype)), int(t1), ws.data_ptr(), size, current_stream_ptr())
+    if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad or topk_weights.requires_grad):
+        out, = refuse_gradient("moe_forward has no backward pass: train with GroupedLinear", out)
     return out
