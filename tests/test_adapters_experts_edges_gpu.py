@@ -9,8 +9,10 @@ if torch.cuda.is_available():
     import test_lora_gpu as lora_tests
     import test_moe_gpu as moe_tests
     from transformer_engine_amd._lib import api, kBFloat16
+    from transformer_engine_amd.linear import linear_backward, linear_forward
     from transformer_engine_amd.lora import LoRALinear, lora, lora_backward, lora_forward
     from transformer_engine_amd.moe import moe_forward, moe_topk
+    from transformer_engine_amd.recipe import DelayedScaling, Float8CurrentScaling, MXFP8BlockScaling
     from transformer_engine_amd.tensor import current_stream_ptr
 
 
@@ -127,3 +129,45 @@ def test_expert_layers_do_not_lose_gradients():
     assert torch.equal(top, want[0]) and torch.equal(w, want[1]) and not top.requires_grad
     with pytest.raises(RuntimeError, match="moe_topk"):
         w.sum().backward()
+
+
+@pytest.mark.parametrize("recipe", ["delayed", "current", "mxfp8"])
+def test_a_frozen_projection_holds_nothing_that_backward_does_not_read(recipe):
+    rec = {"delayed": DelayedScaling, "current": Float8CurrentScaling, "mxfp8": MXFP8BlockScaling}[recipe]
+    t, k, o, r = 4096, 2048, 1024, 8
+    m = LoRALinear(k, o, rank=r, recipe=rec())
+    torch.nn.init.normal_(m.lora_b, std=0.1)
+    ids = torch.zeros(t, dtype=torch.int32, device="cuda")
+    for needs_dx in (True, False):
+        x = torch.randn(t, k, device="cuda", dtype=torch.bfloat16, requires_grad=needs_dx)
+        m(x, ids)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = m(x, ids)
+        held = torch.cuda.memory_allocated() - before
+        # y, the partial rank vectors and, where dx is wanted, the weight's FP8 copies; x's would add t * k = 8 MB
+        weight = (2 * k * o + k * o // 8) * needs_dx
+        low = api.nvte_amd_lora_num_slices(t, k) * t * r * 4
+        assert held <= 2 * t * o + low + weight + (1 << 20), (held, weight)
+        dy = torch.randn_like(y)
+        y.backward(dy)
+        assert (x.grad is not None) == needs_dx and m.lora_a.grad is not None
+
+
+@pytest.mark.parametrize("recipe", ["current", "mxfp8"])
+def test_gradients_beside_a_frozen_projection_are_the_bare_passes(recipe):
+    rec = {"current": Float8CurrentScaling, "mxfp8": MXFP8BlockScaling}[recipe]
+    m = LoRALinear(256, 384, rank=8, num_adapters=3, recipe=rec())
+    torch.nn.init.normal_(m.lora_b, std=0.1)
+    x = torch.randn(64, 256, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    ids = torch.randint(-1, 3, (64,), device="cuda", dtype=torch.int32)
+    y = m(x, ids)
+    dy = torch.randn_like(y)
+    y.backward(dy)
+    with torch.no_grad():
+        base, q = linear_forward(x, m.linear.weight, m.linear.bias, m.linear.fp8_state)
+        want, saved = lora_forward(x, m.lora_a, m.lora_b, ids, m.scaling, base=base)
+        base_grad, _, _ = linear_backward(dy, q, m.linear.fp8_state)
+        dx, da, db = lora_backward(dy, saved, base_grad=base_grad)
+    for got, w in ((y, want), (x.grad, dx), (m.lora_a.grad, da), (m.lora_b.grad, db)):
+        assert torch.equal(got, w)

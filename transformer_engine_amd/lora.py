@@ -200,8 +200,10 @@ class _LoRALinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, adapter_ids, scaling, module):
         lin = module.linear
-        base, ctx.saved_q = linear_forward(x, lin.weight, lin.bias, lin.fp8_state, is_first_microbatch=module._is_first_microbatch,
-                                           needs_backward=module._needs_backward)
+        base, (_, w8) = linear_forward(x, lin.weight, lin.bias, lin.fp8_state, is_first_microbatch=module._is_first_microbatch,
+                                       needs_backward=module._needs_backward)
+        # x's FP8 copy is the weight gradient's, which a frozen weight has not
+        ctx.saved_q = (None, w8) if ctx.needs_input_grad[0] else None
         y, saved = lora_forward(x, a, b, adapter_ids, scaling, base=base, out=base)
         _save(ctx, saved)
         ctx.module = module
