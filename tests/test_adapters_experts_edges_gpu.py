@@ -171,3 +171,19 @@ def test_gradients_beside_a_frozen_projection_are_the_bare_passes(recipe):
         dx, da, db = lora_backward(dy, saved, base_grad=base_grad)
     for got, w in ((y, want), (x.grad, dx), (m.lora_a.grad, da), (m.lora_b.grad, db)):
         assert torch.equal(got, w)
+
+
+def test_casting_a_module_keeps_the_scaling_exact():
+    m = LoRALinear(64, 96, rank=20, alpha=16.0, num_adapters=2)          # 0.8: not a bf16 value
+    x = torch.randn(32, 64, device="cuda", dtype=torch.bfloat16)
+    ids = torch.randint(-1, 2, (32,), device="cuda", dtype=torch.int32)
+    torch.nn.init.normal_(m.lora_b)
+    want = m(x, ids)
+    for cast in (lambda: m.to(torch.bfloat16), m.bfloat16, lambda: torch.nn.Sequential(m).to("cuda", torch.bfloat16)):
+        cast()
+        assert m.scaling.dtype == torch.float32 and (m.scaling == torch.tensor(0.8)).all()
+    assert m.state_dict()["scaling"].dtype == torch.float32
+    got = m(x, ids)
+    assert got.dtype == want.dtype and torch.isfinite(got.float()).all()
+    m.half()
+    assert m.scaling.dtype == torch.float32 and m(x.half(), ids).dtype == torch.float16

@@ -246,6 +246,13 @@ class LoRALinear(torch.nn.Module):
         self.register_buffer("scaling", torch.full((num_adapters,), (rank if alpha is None else alpha) / rank,
                                                    dtype=torch.float32, device=device))
 
+    def _apply(self, fn, *args, **kwargs):
+        scaling = self.scaling
+        super()._apply(fn, *args, **kwargs)
+        if self.scaling.dtype != torch.float32:     # a cast of the parameters leaves the factor as it was
+            self.scaling = scaling.to(self.scaling.device)
+        return self
+
     def forward(self, x: torch.Tensor, adapter_ids: Optional[torch.Tensor] = None,
                 is_first_microbatch: Optional[bool] = None) -> torch.Tensor:
         if adapter_ids is None:
