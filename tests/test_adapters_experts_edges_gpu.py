@@ -8,6 +8,7 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     import test_lora_gpu as lora_tests
     import test_moe_gpu as moe_tests
+    from transformer_engine_amd import NVTEError
     from transformer_engine_amd._lib import api, kBFloat16
     from transformer_engine_amd.linear import linear_backward, linear_forward
     from transformer_engine_amd.lora import LoRALinear, lora, lora_backward, lora_forward
@@ -187,3 +188,18 @@ def test_casting_a_module_keeps_the_scaling_exact():
     assert got.dtype == want.dtype and torch.isfinite(got.float()).all()
     m.half()
     assert m.scaling.dtype == torch.float32 and m(x.half(), ids).dtype == torch.float16
+
+
+def test_many_adapters_beside_a_wide_projection():
+    """More matrices to transpose than one launch has workgroups for."""
+    t, k, o, r, n = 5, 16, 65536, 1, 4096
+    x, a, b, _, s, _, dy, _ = lora_tests.make(t, k, o, r, n, torch.bfloat16)
+    ids = torch.tensor([0, 4095, -1, 2048, 4095], dtype=torch.int32, device="cuda")
+    y, saved = lora_forward(x, a, b, ids, s)
+    dx, da, db = lora_backward(dy, saved)
+    assert torch.equal(lora_backward(dy, saved, requires_wgrad=False)[0], dx)
+    used = [0, 2048, 4095]
+    few = torch.tensor([0, 2, -1, 1, 2], device="cuda")
+    lora_tests.check_all((x, a[used], b[used], few, s[used], None, dy, None), y, dx, da[used], db[used])
+    for grad in (da, db):
+        assert (grad.flatten(1).abs().sum(1) > 0).nonzero().flatten().tolist() == used

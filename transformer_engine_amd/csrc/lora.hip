@@ -445,6 +445,7 @@ struct PrepareArgs {
   Plan plan;
   int64_t tokens;
   int features, rank, num, per_item, lists;  // lists: workgroups of the first part, num + 1 or none
+  int64_t pieces;                            // of the second part, dealt out over its workgroups
 };
 
 __device__ __forceinline__ int sum_1024(int v, int *scratch) {  // valid in every thread
@@ -555,8 +556,16 @@ __global__ __launch_bounds__(1024) void prepare_kernel(PrepareArgs p) {
     uint16_t rows[64 * (kMaxRank + 1)];
   } s;
   __shared__ int scratch[16];
-  if (static_cast<int>(blockIdx.x) < p.lists) list_tokens(p, blockIdx.x, s.hist, scratch);
-  else transpose_rows(p, blockIdx.x - p.lists, s.rows);
+  if (static_cast<int>(blockIdx.x) < p.lists) {
+    list_tokens(p, blockIdx.x, s.hist, scratch);
+    return;
+  }
+  for (int64_t piece = blockIdx.x - p.lists;;) {
+    transpose_rows(p, piece, s.rows);
+    piece += gridDim.x - p.lists;
+    if (piece >= p.pieces) return;
+    __syncthreads();  // the last piece is written
+  }
 }
 
 // ====================================================================================
@@ -909,10 +918,10 @@ int64_t most_items(const Shape &s) {
 // one launch: the lists, if wanted, and B transposed, if given
 void prepare(const Shape &s, const int *ids, const Plan &plan, bool lists, const void *b, uint16_t *transposed, hipStream_t stream) {
   const int64_t pieces = b != nullptr ? static_cast<int64_t>(s.num) * ceil_div(s.out, 64) : 0, first = lists ? s.num + 1 : 0;
-  NVTE_CHECK(first + pieces < (1 << 22), "too many adapters to transpose: ", s.num);
   const PrepareArgs p{ids, static_cast<const uint16_t *>(b), transposed, plan, s.tokens, s.out, s.rank, s.num, blocks_per_item(s),
-                      static_cast<int>(first)};
-  hipLaunchKernelGGL(prepare_kernel, dim3(first + pieces), dim3(1024), 0, stream, p);
+                      static_cast<int>(first), pieces};
+  // a launch has fewer than 2^32 threads
+  hipLaunchKernelGGL(prepare_kernel, dim3(first + std::min<int64_t>(pieces, 1 << 21)), dim3(1024), 0, stream, p);
   NVTE_CHECK_HIP(hipGetLastError());
 }
 
