@@ -74,3 +74,9 @@ def test_workspace_of_a_pass_without_weight_gradients_is_checked_by_its_own_size
             _backward(**bad)
     assert api.nvte_amd_lora_dgrad_workspace_size(0, 14336, 16, 512) == 0
     _backward(0, 0, da=0, db=0, tokens=0)               # nothing to do, nothing launched
+
+
+def test_router_refuses_more_tokens_than_a_launch_has_threads_for():
+    for tokens in ((1 << 26) - 3, 1 << 26, 1 << 40):
+        with pytest.raises(NVTEError, match="too many tokens"):
+            api.nvte_amd_moe_topk(P, P, P, tokens, 8, 2, 1, kFloat32, 0)

@@ -584,7 +584,7 @@ void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, s
     NVTE_CHECK(num_experts >= 1 && num_experts <= kMaxExperts, "number of experts must be 1 to ", kMaxExperts, ", got ", num_experts);
     NVTE_CHECK(top_k >= 1 && top_k <= 64 && top_k <= num_experts, "top_k must be 1 to 64 and at most the number of experts (",
                num_experts, "), got ", top_k);
-    NVTE_CHECK(tokens < (1u << 26), "too many tokens: ", tokens);
+    NVTE_CHECK(tokens <= (1u << 26) - 4, "too many tokens: ", tokens);  // 64 threads each, fewer than 2^32 in a launch
     if (tokens == 0) return;
     NVTE_CHECK(logits && topk_ids && topk_weights, "a required pointer is NULL");
     auto launch_topk = [&](auto kernel) {
