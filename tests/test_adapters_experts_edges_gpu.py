@@ -203,3 +203,24 @@ def test_many_adapters_beside_a_wide_projection():
     lora_tests.check_all((x, a[used], b[used], few, s[used], None, dy, None), y, dx, da[used], db[used])
     for grad in (da, db):
         assert (grad.flatten(1).abs().sum(1) > 0).nonzero().flatten().tolist() == used
+
+
+def test_the_largest_number_of_tokens():
+    t, k, o, r = 1 << 27, 4, 8, 1
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(t, k, generator=g, device="cuda", dtype=torch.bfloat16)
+    dy = torch.randn(t, o, generator=g, device="cuda", dtype=torch.bfloat16)
+    a, b = torch.randn(1, r, k, device="cuda", dtype=torch.bfloat16), torch.randn(1, o, r, device="cuda", dtype=torch.bfloat16)
+    ids = torch.full((t,), -1, dtype=torch.int32, device="cuda")
+    rows = torch.cat([torch.arange(100, device="cuda"), torch.randint(0, t, (800,), generator=g, device="cuda"),
+                      torch.arange(t - 100, t, device="cuda")]).unique()
+    ids[rows] = 0
+    y, saved = lora_forward(x, a, b, ids)
+    dx, da, db = lora_backward(dy, saved)
+    one = torch.zeros(len(rows), dtype=torch.int32, device="cuda")
+    lora_tests.check_all((x[rows], a, b, one, None, None, dy[rows], None), y[rows], dx[rows], da, db)
+    for v in (y, dx):
+        v[rows] = 0
+        assert v.count_nonzero() == 0
+    with pytest.raises(NVTEError, match="tokens"):
+        lora_forward(torch.cat([x, x[:1]]), a, b, torch.cat([ids, ids[:1]]))

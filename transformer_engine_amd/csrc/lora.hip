@@ -607,10 +607,11 @@ template <typename E, int KT, int MT, bool SMALL>
 __global__ __launch_bounds__(256, KT == 1 ? 2 : 1) void expand_pack_kernel(ExpandArgs p, PackArgs q, int column_ranges, int tiles, int phases,
                                                           int blocks) {
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[16 * MT][KT * 32 + 8], s_lo[16 * MT][KT * 32 + 8];
-  const int b = blockIdx.x;
+  const int b = blockIdx.x + gridDim.x * blockIdx.y;
   if (b < 2 * blocks) pack_block(q, b < blocks ? q.side[0] : q.side[1], b < blocks ? b : b - blocks);
   else {
     const int n = (b - 2 * blocks) / tiles;
+    if (n >= column_ranges * phases) return;
     expand_tile<E, KT, MT, true, SMALL>(p, (b - 2 * blocks) % tiles, n % column_ranges, n / column_ranges, phases, s_hi, s_lo);
   }
 }
@@ -886,10 +887,9 @@ void expand_and_pack(ExpandArgs p, const PackArgs &q, int64_t blocks, hipStream_
     p.cols = columns_of(tiles, p.features);
     const int64_t ranges = p.out != nullptr ? ceil_div(p.features, p.cols) : 0;
     const int phases = p.plan.order != nullptr ? 1 : phases_of(std::max<int64_t>(1, tiles * ranges), p.tokens, p.num);
-    const int64_t grid = 2 * blocks + tiles * ranges * phases;
-    NVTE_CHECK(grid < (1 << 24), "too many workgroups: ", grid);
-    if (grid == 0) return;
-    hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt(), small()>), dim3(grid), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
+    const int64_t all = 2 * blocks + tiles * ranges * phases, grid = std::min<int64_t>(all, 1 << 23);  // fewer than 2^32 threads along x
+    if (all == 0) return;
+    hipLaunchKernelGGL((expand_pack_kernel<E, kt(), mt(), small()>), dim3(grid, ceil_div(all, grid)), dim3(256), 0, stream, p, q, static_cast<int>(ranges),
                        static_cast<int>(tiles), phases, static_cast<int>(blocks));
     NVTE_CHECK_HIP(hipGetLastError());
   });
