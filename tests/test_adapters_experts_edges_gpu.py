@@ -15,6 +15,7 @@ if torch.cuda.is_available():
     from transformer_engine_amd.moe import moe_forward, moe_topk
     from transformer_engine_amd.recipe import DelayedScaling, Float8CurrentScaling, MXFP8BlockScaling
     from transformer_engine_amd.tensor import current_stream_ptr
+    from transformer_engine_amd.weight_update import clip_grad_norm, grad_norm
 
 
 @pytest.mark.parametrize("t, n", [(3, 5), (40, 300), (700, 6), (700, 1), (520, 5000)])
@@ -224,3 +225,125 @@ def test_the_largest_number_of_tokens():
         assert v.count_nonzero() == 0
     with pytest.raises(NVTEError, match="tokens"):
         lora_forward(torch.cat([x, x[:1]]), a, b, torch.cat([ids, ids[:1]]))
+
+
+def _work(seed):
+    """One user's module, requests, experts and gradients, unlike another's, and a step through all of them: decode of 33 tokens, a training
+    batch long enough to be ordered by adapter, clipping."""
+    torch.manual_seed(seed)
+    m = LoRALinear(256, 192, rank=8, num_adapters=4, recipe=Float8CurrentScaling())
+    torch.nn.init.normal_(m.lora_b, std=0.1)
+    x = torch.randn(33, 256, device="cuda", dtype=torch.bfloat16)
+    ids = torch.randint(-1, 4, (33,), device="cuda", dtype=torch.int32)
+    router = torch.randn(192, 16, device="cuda") * 192 ** -0.5
+    _, w1, w2, _, _, s1, s2 = moe_tests.make(1, 192, 136, 16, 2, torch.bfloat16, fp8=True, seed=seed)
+    xt, a, b, it, s, base, dy, gbase = lora_tests.make(1400, 264, 392, 16, 5, torch.bfloat16, seed=seed)
+    outs = [torch.empty_like(v, dtype=torch.float32) for v in (a, b)]
+    def step():
+        with torch.no_grad():
+            h = m(x, ids)
+        top, weights = moe_topk(h.float() @ router, 2)
+        out = moe_forward(h, w1, w2, top, weights, s1, s2)
+        y, saved = lora_forward(xt, a, b, it, s, base=base)
+        dx, da, db = lora_backward(dy, saved, base_grad=gbase)
+        few = lora_backward(dy, saved, requires_wgrad=False)[0]
+        norm = clip_grad_norm([da, db], 1.0, outs=outs)
+        return [v.clone() for v in (h, top, weights, out, y, dx, da, db, few, norm, *outs)]
+    return step
+
+
+def test_two_users_on_two_streams():
+    steps = [_work(1), _work(2)]
+    want = [step() for step in steps]
+    torch.cuda.synchronize()
+    assert not any(torch.equal(p, q) for p, q in zip(*want))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for s, step, g in zip(streams, steps, got):
+            with torch.cuda.stream(s):
+                g.append(step())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for outs in g:
+            assert all(torch.equal(p, q) for p, q in zip(outs, w))
+
+
+def test_two_users_in_two_graphs_at_once():
+    steps = [_work(3), _work(4)]
+    want = [step() for step in steps]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, held = [], []
+    for step, s in zip(steps, streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step())
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for outs in held:
+            for v in outs:
+                v.zero_()
+        steps[0]()                                   # a third user between the replays
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for outs, w in zip(held, want):
+            assert all(torch.equal(p, q) for p, q in zip(outs, w))
+
+
+def _rank_grads(rank):
+    """Every rank another list: lengths, dtypes and sizes of its own, the last rank none at all."""
+    g = torch.Generator(device="cuda").manual_seed(100 + rank)
+    lengths, std = ([5000, 17], [40_001, 1, 333], [])[rank], (1.0, 30.0, 0.0)[rank]
+    return [(torch.randn(n, generator=g, device="cuda") * std).to((torch.bfloat16, torch.float32)[(i + rank) % 2])
+            for i, n in enumerate(lengths)]
+
+
+def _clip_over_ranks(rank, world, port, ret):
+    import os
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.cuda.set_device(0)
+        everyone = [v.double().square().sum().item() for r in range(world) for v in _rank_grads(r)]
+        want = sum(everyone) ** 0.5
+        grads = _rank_grads(rank)
+        keep = [v.clone() for v in grads]
+        assert abs(grad_norm(grads, group=dist.group.WORLD).item() - want) <= want * 2.0 ** -23
+        for outs in ([torch.empty_like(v, dtype=torch.float32) for v in grads], None):
+            norm = clip_grad_norm(grads, 2.0, outs=outs, group=dist.group.WORLD)
+            assert norm.shape == (1,) and abs(norm.item() - want) <= want * 2.0 ** -23
+            for k, o in zip(keep, grads if outs is None else outs):
+                exact = k.double() * (2.0 / (want + 1e-6))
+                assert ((o.double() - exact).abs() <= exact.abs() * (torch.finfo(o.dtype).eps / 2 + 2.0 ** -22) + 1e-38).all()
+        bits = torch.tensor([norm.item()], dtype=torch.float64)
+        low, high = bits.clone(), bits.clone()
+        dist.all_reduce(low, op=dist.ReduceOp.MIN)
+        dist.all_reduce(high, op=dist.ReduceOp.MAX)
+        assert low == high == bits
+        ret[rank] = "ok"
+    except Exception:
+        import traceback
+        ret[rank] = traceback.format_exc()
+    finally:
+        dist.destroy_process_group()
+
+
+def test_norm_and_clip_over_three_ranks():
+    import socket
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ret = mp.get_context("spawn").Manager().dict()
+    mp.spawn(_clip_over_ranks, args=(3, port, ret), nprocs=3, join=True)
+    assert dict(ret) == {0: "ok", 1: "ok", 2: "ok"}, dict(ret)
