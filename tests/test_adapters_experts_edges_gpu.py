@@ -347,3 +347,15 @@ def test_norm_and_clip_over_three_ranks():
     ret = mp.get_context("spawn").Manager().dict()
     mp.spawn(_clip_over_ranks, args=(3, port, ret), nprocs=3, join=True)
     assert dict(ret) == {0: "ok", 1: "ok", 2: "ok"}, dict(ret)
+
+
+@pytest.mark.parametrize("ids", ["mixed", "runs"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,k,o,r,n", [(512, 136, 264, 16, 400), (1500, 72, 104, 40, 1000), (5000, 264, 136, 16, 3000), (4100, 7, 12, 5, 4096)])
+def test_many_adapters_for_the_tokens_at_hand(t, k, o, r, n, dtype, ids):
+    x, a, b, i, s, base, dy, gbase = lora_tests.make(t, k, o, r, n, dtype, seed=t, ids=ids, std=0.5)
+    y, saved = lora_forward(x, a, b, i, s, base=base)
+    dx, da, db = lora_backward(dy, saved, base_grad=gbase)
+    lora_tests.check_all((x, a, b, i, s, base, dy, gbase), y, dx, da, db)
+    alone = lora_backward(dy, saved, base_grad=gbase, requires_wgrad=False)[0]
+    lora_tests.check_all((x, a, b, i, s, base, dy, gbase), y, alone, da, db)

@@ -80,3 +80,11 @@ def test_router_refuses_more_tokens_than_a_launch_has_threads_for():
     for tokens in ((1 << 26) - 3, 1 << 26, 1 << 40):
         with pytest.raises(NVTEError, match="too many tokens"):
             api.nvte_amd_moe_topk(P, P, P, tokens, 8, 2, 1, kFloat32, 0)
+
+
+def test_batches_are_put_in_order_only_where_their_pool_is_small_beside_them():
+    size = api.nvte_amd_lora_forward_workspace_size
+    for tokens, adapters in ((511, 2), (512, 1), (512, 257), (512, 4096), (1024, 1024), (8191, 4096), (1 << 20, 4097)):
+        assert size(tokens, adapters) == 0, (tokens, adapters)
+    for tokens, adapters in ((512, 2), (512, 256), (2048, 1024), (8192, 4096)):
+        assert size(tokens, adapters) > tokens * 4, (tokens, adapters)

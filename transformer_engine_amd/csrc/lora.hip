@@ -812,10 +812,18 @@ int64_t tiles_of(const Plan &plan, int64_t tokens, int num, int size) {
   return plan.order != nullptr ? most_blocks(tokens, num) * kBlock / size : static_cast<int64_t>(ceil_div(tokens, size));
 }
 
-// Tokens are put in order of their adapters first where tiles would otherwise walk through many.  In any order, 8192 x (8192 -> 14336) with 64
-// adapters of rank 8 took 1356 us without and 168 us with it, 600 x (4096 -> 4096) with 32 of rank 16 46 and 23 us; a batch whose
-// requests lie back to back pays the extra launch (23 and 28 us at the latter size), and below 512 tokens both orders lose.
-bool ordered(int64_t tokens, int num) { return tokens >= 512 && num > 1 && num <= kMaxAdapters; }
+// Tokens are put in order of their adapters first where tiles would otherwise walk through many, and where listing them costs less than
+// that: `prepare` reads all ids once for every adapter.  A forward pass of 4096 -> 4096, rank 16, ids in any order, in us with / without:
+//   adapters   512 tokens    1024         2048         4096         8192
+//   64         30 / 44       31 / 76      40 / 135     63 / 320     97 / 631
+//   256        52 / 46       54 / 88      61 / 153     76 / 372     123 / 737
+//   1024       88 / 52       115 / 98     133 / 162    153 / 380    183 / 762
+//   4096       125 / 59      164 / 110    248 / 167    354 / 379    462 / 771
+// Requests that lie back to back pay for nothing (2048 tokens of 64: 39 / 36; 4096 of 4096: 354 / 281); below 512 tokens both orders lose.
+// A pass that lists the tokens anyway, for its weight gradients, follows the lists.
+bool ordered(int64_t tokens, int num, bool listed) {
+  return tokens >= 512 && num > 1 && num <= kMaxAdapters && (listed || tokens >= 2ll * num);
+}
 
 template <typename E, int RT, int MT, int NW, int U, bool SMALL = false>
 void launch_shrink(const ShrinkArgs &p, int slices, hipStream_t stream) {
@@ -942,7 +950,7 @@ struct ForwardWorkspace {
   }
 };
 ForwardWorkspace forward_workspace(int64_t tokens, int num) {
-  if (!ordered(tokens, num)) return {};
+  if (!ordered(tokens, num, false)) return {};
   ForwardWorkspace w{};
   Space space;
   w.order = space.take(most_blocks(tokens, num) * kBlock * sizeof(int));
@@ -968,7 +976,7 @@ BackwardWorkspace backward_workspace(const Shape &s, bool wgrad) {
   Space space;
   auto take = [&](size_t bytes) { return space.take(bytes); };
   w.wgrad = wgrad;
-  w.lists = wgrad || ordered(s.tokens, s.num);
+  w.lists = wgrad || ordered(s.tokens, s.num, false);
   w.low = take(static_cast<size_t>(num_slices(s.tokens, s.out)) * s.tokens * s.rank * sizeof(float));
   w.transposed = take(s.tokens > 0 ? static_cast<size_t>(s.num) * s.rank * s.out * 2 : 0);
   if (w.lists) {
@@ -992,14 +1000,14 @@ BackwardWorkspace backward_workspace(const Shape &s, bool wgrad) {
 template <typename E>
 void backward(const Shape &s, const void *x, const void *dy, const void *a, const void *b, const int *ids, const float *scaling,
               const float *low, const void *base_grad, void *dx, void *da, void *db, int grad_type, char *ws, hipStream_t stream) {
-  const bool wgrad = da != nullptr, in_order = ordered(s.tokens, s.num);
+  const bool wgrad = da != nullptr;
   if (!wgrad && (dx == nullptr || s.tokens == 0)) return;
   const BackwardWorkspace w = backward_workspace(s, wgrad);
   float *up = reinterpret_cast<float *>(ws + w.low);
   uint16_t *bt = reinterpret_cast<uint16_t *>(ws + w.transposed);
   const Plan plan = w.plan(ws);
   prepare(s, ids, plan, w.lists, s.tokens > 0 ? b : nullptr, bt, stream);
-  const Plan tiles = in_order ? plan : Plan{};
+  const Plan tiles = ordered(s.tokens, s.num, wgrad) ? plan : Plan{};
   const int64_t blocks = wgrad ? most_blocks(s.tokens, s.num) : 0;
   uint16_t *packed_a = reinterpret_cast<uint16_t *>(ws + w.packed_a), *packed_b = reinterpret_cast<uint16_t *>(ws + w.packed_b);
   if (s.tokens > 0) {
