@@ -132,7 +132,7 @@ void nvte_amd_lora_backward(const void *x, const void *dy, const void *a, const 
                             int dtype, int grad_dtype, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ---- A mixture-of-experts layer for a few tokens (Python: moe.py); larger batches: the grouped GEMM.
- * Router: p = softmax(logits[t]) over num_experts (<= 1024) fp32 / fp16 / bf16 logits; topk_ids [tokens, top_k] int32 = the largest,
+ * Router (up to 2^26 - 4 tokens): p = softmax(logits[t]) over num_experts (<= 1024) fp32 / fp16 / bf16 logits; topk_ids [tokens, top_k] int32 = the largest,
  * in falling order, ties to the lowest index, NaN last; topk_weights fp32 = p of them, divided by their sum if renormalize. */
 void nvte_amd_moe_topk(const void *logits, int *topk_ids, float *topk_weights, size_t tokens, size_t num_experts, size_t top_k,
                        int renormalize, int dtype, hipStream_t stream);
